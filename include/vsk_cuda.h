@@ -534,6 +534,44 @@ int32_t vsk_pq_index_create(vsk_ctx* ctx, int32_t dim, int32_t segments, int32_t
 int32_t vsk_pq_index_add(vsk_index* index, const uint8_t* codes, int64_t n);
 int32_t vsk_pq_index_add_dev(vsk_index* index, const uint8_t* codes, int64_t n);
 
+/* --- rows in four bits -----------------------------------------------------------------------
+ * The next step below the int8 quantiser: a scale, and optionally a middle, per group of 32, 64 or 128 columns of a row
+ * (ScalarQuantizer has one scale for the whole batch, Quantization/ScalarQuantizer.swift:389-451).  A group of the last
+ * columns may be shorter.  Per group, with lo, hi and the largest magnitude amax of its values, in 64 bits:
+ *   symmetric   s = half(float(amax / 7))                                   value = s (c - 8)
+ *   min / max   s = half(float((hi - lo) / 15)), m = half(float(lo + 8 s))   value = s (c - 8) + m
+ *   code        c = clip(nearest((x - m) / s) + 8, 0, 15), the quotient in 64 bits, ties to even; c = 8 where s = 0
+ * (half: rounded to fp16; s at most 65 504, m within +-65 504).  The values to encode are finite.
+ *   codes       [n] rows of code_stride bytes, two codes a byte, the even column in the low four bits; the high half of an odd
+ *               last column is 8.  Bytes behind a row's columns are neither read nor written.
+ *   scales, middles   [n] rows of scale_stride fp16 numbers, one per group; encoding writes them dense (stride = groups)
+ * Element types of the `void*` arguments: vsk_dtype.  Strides count elements, code_stride bytes.
+ *   encode      rows[n][row_stride] -> codes, scales, middles (NULL with symmetric != 0)
+ *   decode      -> out[n][dim] fp32, each value rounded once
+ *   product     y[q * y_stride + r] = sum over the columns of value(r, i) x[q * x_stride + i]: the scores of nq vectors
+ *               against all rows, as a decoding step takes them from a projection or an output head, or a query from a store
+ *               (dotProduct negates them).  Sums in fp32, rounded once to y's type.  fp32 vectors are taken exactly.  Finite vectors
+ *               with elements below 2^120.  x and y must not overlap. */
+typedef enum vsk_dtype { VSK_DTYPE_F32 = 0, VSK_DTYPE_F16 = 1, VSK_DTYPE_BF16 = 2 } vsk_dtype;
+typedef struct vsk_q4_rows {
+  const uint8_t* codes;
+  const void* scales;      /* fp16 */
+  const void* middles;     /* fp16, or NULL: symmetric */
+  int64_t code_stride;     /* bytes */
+  int64_t scale_stride;    /* fp16 numbers */
+  int64_t n;
+  int32_t dim;
+  int32_t group;           /* 32, 64 or 128 */
+} vsk_q4_rows;
+int32_t vsk_q4_encode(vsk_ctx* ctx, const float* rows, int64_t n, int32_t dim, int32_t group, int32_t symmetric, uint8_t* codes,
+                      int64_t code_stride, void* scales, void* middles);
+int32_t vsk_q4_encode_dev(vsk_ctx* ctx, const void* rows, int32_t dtype, int64_t n, int32_t dim, int64_t row_stride, int32_t group,
+                          int32_t symmetric, uint8_t* codes, int64_t code_stride, void* scales, void* middles);
+int32_t vsk_q4_decode(vsk_ctx* ctx, const vsk_q4_rows* rows, float* out);
+int32_t vsk_q4_decode_dev(vsk_ctx* ctx, const vsk_q4_rows* rows, float* out);
+int32_t vsk_q4_product_dev(vsk_ctx* ctx, const vsk_q4_rows* rows, const void* x, int32_t x_dtype, int64_t nq, int64_t x_stride,
+                           void* y, int32_t y_dtype, int64_t y_stride);
+
 #ifdef __cplusplus
 }
 #endif

@@ -50,6 +50,12 @@ class Tuning(C.Structure):
                 ("stage_kblocks", C.c_int32), ("reserved", C.c_int32 * 6)]
 
 
+class Q4Rows(C.Structure):
+    _fields_ = [("codes", vp), ("scales", vp), ("middles", vp), ("code_stride", C.c_int64), ("scale_stride", C.c_int64),
+                ("n", C.c_int64), ("dim", C.c_int32), ("group", C.c_int32)]
+
+
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2   # vsk_dtype
 COMM_ID_BYTES = 128
 SHARDED_SLICE, SHARDED_ALL, SHARDED_QUERIES_SPLIT = 0, 1, 16
 SHARDED_PHASES = 7
@@ -153,6 +159,11 @@ SIGNATURES = {
     "vsk_sq8_index_create": (C.c_int32, [vp, C.c_int32, C.c_int32, vp, vp, C.POINTER(vp)]),
     "vsk_sq8_index_add": (C.c_int32, [vp, vp, C.c_int64]),
     "vsk_sq8_index_add_dev": (C.c_int32, [vp, vp, C.c_int64]),
+    "vsk_q4_encode": (C.c_int32, [vp, vp, C.c_int64, C.c_int32, C.c_int32, C.c_int32, vp, C.c_int64, vp, vp]),
+    "vsk_q4_encode_dev": (C.c_int32, [vp, vp, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_int32, C.c_int32, vp, C.c_int64, vp, vp]),
+    "vsk_q4_decode": (C.c_int32, [vp, C.POINTER(Q4Rows), vp]),
+    "vsk_q4_decode_dev": (C.c_int32, [vp, C.POINTER(Q4Rows), vp]),
+    "vsk_q4_product_dev": (C.c_int32, [vp, C.POINTER(Q4Rows), vp, C.c_int32, C.c_int64, C.c_int64, vp, C.c_int32, C.c_int64]),
 }
 
 _lib = None

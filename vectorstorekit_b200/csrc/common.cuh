@@ -9,6 +9,7 @@
 
 #include <functional>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include <nvtx3/nvToolsExt.h>   // header-only; ranges cost nothing unless a profiler is attached
@@ -204,6 +205,7 @@ struct Ctx {
   PinnedBuf host_flags[2];   // per lane: the flag words a finished half-search hands to the host
   std::vector<const void*> configured;   // kernels that have their shared memory on this device (opt_in_shared) ...
   std::vector<const void*> carved;       // ... and first ones of groups with the carve-out (prefer_shared_carveout)
+  std::vector<std::pair<const void*, int>> resident;   // blocks of a kernel that fit an SM of this device (resident_blocks)
   unsigned* few_tickets[2] = {};   // per lane: the few-query search's tickets (few_search.cu)
   Comm* comm = nullptr;
   Worker* worker = nullptr;
@@ -251,6 +253,21 @@ inline cudaError_t opt_in_shared(Ctx* ctx, K kernel, size_t bytes) {
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (e == cudaSuccess) ctx->configured.push_back((const void*)kernel);
   return e;
+}
+
+// Blocks of a kernel that one SM holds, always asked with the same block and shared memory: once per context.
+template <typename K>
+inline int resident_blocks(Ctx* ctx, K kernel, int threads, size_t shared) {
+  for (const auto& r : ctx->resident)
+    if (r.first == (const void*)kernel) return r.second;
+  int blocks = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, threads, shared) != cudaSuccess) {
+    cudaGetLastError();
+    blocks = 1;
+  }
+  if (blocks < 1) blocks = 1;
+  ctx->resident.push_back({(const void*)kernel, blocks});
+  return blocks;
 }
 
 // Issues on lane `lane` until it goes out of scope.

@@ -1,0 +1,179 @@
+"""Rows in four bits with a scale per group of columns: the quantiser and the products of vectors with such rows.
+
+``Int4Quantizer`` stands beside ``ScalarQuantizer`` (int8, one scale per column or per matrix;
+``Quantization/ScalarQuantizer.swift:129-164``).  The format is stated in ``include/vsk_cuda.h``.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+from . import _lib
+from .engine import (CUDAComputeDevice, DimensionMismatch, EmptyInput, InvalidBufferSize, InvalidInput, UnsupportedOperation, _host,
+                     _is_dev, _ptr)
+
+try:  # torch is plumbing for device memory only
+    import torch
+except Exception:  # pragma: no cover
+    torch = None
+
+
+def _dtype_id(t) -> int:
+    """``vsk_dtype`` of a torch element type."""
+    ids = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+    if t not in ids:
+        raise UnsupportedOperation(f"element type {t} is not supported (float32, float16 or bfloat16)")
+    return ids[t]
+
+
+def _span(t) -> int:
+    """Bytes from a tensor's first element to its last."""
+    if t.numel() == 0:
+        return 0
+    return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _device_pointers(dev: CUDAComputeDevice, *tensors):
+    """Addresses of CUDA tensors of the device object's GPU (None stays None).  The library works on its own stream: the current
+    torch stream is waited for once, as every call of this package does."""
+    for t in tensors:
+        if t is not None and (not _is_dev(t) or t.device.index != dev.device):
+            raise InvalidInput(f"expected a CUDA tensor on device {dev.device}, got {t.device if hasattr(t, 'device') else type(t).__name__}")
+    torch.cuda.current_stream(dev.device).synchronize()
+    out = []
+    for t in tensors:
+        if t is not None and _lib.CHECKED and t.numel():
+            dev._lib.vsk_checked_register(C.c_void_p(t.data_ptr()), _span(t))
+        out.append(None if t is None else C.c_void_p(t.data_ptr()))
+    return out
+
+
+def _rows_2d(t, what):
+    """A matrix whose rows are contiguous (they may lie inside wider ones); others are copied."""
+    if t.dim() != 2:
+        raise DimensionMismatch(f"{what} must be a matrix, got {t.dim()} dimensions")
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+def _row_stride(t) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+class Int4Quantizer:
+    """Rows in four bits: two codes a byte and one fp16 scale per ``groupSize`` columns of a row (32, 64 or 128).
+
+    ``symmetric=True``: a value is ``scale * (code - 8)``.  ``symmetric=False``: ``scale * (code - 8) + middle``, for groups whose
+    values do not lie around zero.  There is nothing to train: a group's scale comes from its own values."""
+
+    def __init__(self, dev: CUDAComputeDevice, groupSize: int = 64, symmetric: bool = True):
+        if groupSize not in (32, 64, 128):
+            raise UnsupportedOperation(f"groups of {groupSize} columns are not supported (32, 64 or 128)")
+        self.dev, self._lib = dev, dev._lib
+        self.groupSize, self.symmetric = int(groupSize), bool(symmetric)
+
+    def _groups(self, dim: int) -> int:
+        return -(-dim // self.groupSize)
+
+    def quantizeBatch(self, vectors):
+        """Finite rows ``[n][dim]`` -> ``(codes, scales, middles)``: ``[n][ceil(dim / 2)]`` bytes, ``[n][groups]`` fp16 and the same
+        or None.  CUDA tensors of float32, float16 or bfloat16 give CUDA tensors, whose code rows begin at 16-byte boundaries; host
+        arrays are taken as float32 and give host arrays."""
+        if len(vectors) == 0:
+            raise EmptyInput("no rows")
+        if len(vectors.shape) != 2 or vectors.shape[1] == 0:
+            raise DimensionMismatch("rows must be a matrix with at least one column")
+        n, dim = (int(v) for v in vectors.shape)
+        width, groups, sym = (dim + 1) // 2, self._groups(dim), 1 if self.symmetric else 0
+        if _is_dev(vectors):
+            x = _rows_2d(vectors, "rows")
+            kind = _dtype_id(x.dtype)
+            codes = torch.empty((n, -(-width // 16) * 16), dtype=torch.uint8, device=x.device)[:, :width]
+            scales = torch.empty((n, groups), dtype=torch.float16, device=x.device)
+            middles = None if self.symmetric else torch.empty_like(scales)
+            px, pc, ps, pm = _device_pointers(self.dev, x, codes, scales, middles)
+            self.dev.check(self._lib.vsk_q4_encode_dev(self.dev._h, px, kind, n, dim, _row_stride(x), self.groupSize, sym, pc,
+                                                       _row_stride(codes), ps, pm))
+            return codes, scales, middles
+        x = _host(vectors, np.float32)
+        codes = np.empty((n, width), np.uint8)
+        scales = np.empty((n, groups), np.float16)
+        middles = None if self.symmetric else np.empty((n, groups), np.float16)
+        self.dev.check(self._lib.vsk_q4_encode(self.dev._h, _ptr(x), n, dim, self.groupSize, sym, _ptr(codes), width, _ptr(scales),
+                                               _ptr(middles)))
+        return codes, scales, middles
+
+    def _descriptor(self, codes, scales, middles, dim, pointers, code_stride, scale_stride):
+        r = _lib.Q4Rows()
+        r.codes, r.scales, r.middles = pointers
+        r.code_stride, r.scale_stride = code_stride, scale_stride
+        r.n, r.dim, r.group = codes.shape[0], dim, self.groupSize
+        return r
+
+    def _check(self, codes, scales, middles, dim):
+        if len(codes) == 0:
+            raise EmptyInput("no rows")
+        if dim <= 0:
+            raise DimensionMismatch("dimension must be positive")
+        if self.symmetric != (middles is None):
+            raise InvalidInput("a symmetric quantiser has no middles, the other one has")
+        if len(codes.shape) != 2 or codes.shape[1] != (dim + 1) // 2:
+            raise DimensionMismatch(f"expected {(dim + 1) // 2} bytes of codes per row for {dim} columns, got {tuple(codes.shape)}")
+        want = (codes.shape[0], self._groups(dim))
+        for name, t in (("scales", scales), ("middles", middles)):
+            if t is not None and tuple(t.shape) != want:
+                raise DimensionMismatch(f"expected {name} of shape {want}, got {tuple(t.shape)}")
+
+    def _device_rows(self, codes, scales, middles, dim):
+        """-> (descriptor's arguments, tensors to keep) for codes and scales in device memory"""
+        self._check(codes, scales, middles, dim)
+        for name, t, want in (("codes", codes, torch.uint8), ("scales", scales, torch.float16), ("middles", middles, torch.float16)):
+            if t is not None and (not _is_dev(t) or t.dtype != want):
+                raise InvalidInput(f"{name} must be a CUDA tensor of {want}")
+        codes, scales = _rows_2d(codes, "codes"), _rows_2d(scales, "scales")
+        if middles is not None:
+            middles = _rows_2d(middles, "middles")
+            if _row_stride(middles) != _row_stride(scales):
+                scales, middles = scales.contiguous(), middles.contiguous()
+        return codes, scales, middles
+
+    def dequantizeBatch(self, codes, scales, middles, dimensions: int):
+        """The fp32 values ``[n][dimensions]`` that the codes stand for."""
+        dim = int(dimensions)
+        if _is_dev(codes):
+            codes, scales, middles = self._device_rows(codes, scales, middles, dim)
+            out = torch.empty((codes.shape[0], dim), dtype=torch.float32, device=codes.device)
+            *p, po = _device_pointers(self.dev, codes, scales, middles, out)
+            r = self._descriptor(codes, scales, middles, dim, p, _row_stride(codes), _row_stride(scales))
+            self.dev.check(self._lib.vsk_q4_decode_dev(self.dev._h, C.byref(r), po))
+            return out
+        codes, scales = _host(codes, np.uint8), _host(scales, np.float16)
+        middles = None if middles is None else _host(middles, np.float16)
+        self._check(codes, scales, middles, dim)
+        out = np.empty((codes.shape[0], dim), np.float32)
+        r = self._descriptor(codes, scales, middles, dim, [_ptr(codes), _ptr(scales), _ptr(middles)], codes.shape[1], scales.shape[1])
+        self.dev.check(self._lib.vsk_q4_decode(self.dev._h, C.byref(r), _ptr(out)))
+        return out
+
+    def product(self, x, codes, scales, middles=None, out_dtype=None):
+        """``[queries][n]`` products of vectors ``x [queries][dim]`` with all rows: the logits of an output head, a projection of
+        tokens, or the scores of queries against a store (``DistanceMetric.dotProduct`` is their negative).  Sums in fp32, rounded
+        once to ``out_dtype`` (float32, float16 or bfloat16; default: x's type).  fp32 vectors are taken exactly.  CUDA tensors; no
+        gradient flows."""
+        if not _is_dev(x):
+            raise InvalidInput("product takes CUDA tensors")
+        if x.dim() != 2:
+            raise DimensionMismatch("x must be a matrix of one vector per row")
+        if x.shape[0] == 0:
+            raise EmptyInput("no vectors")
+        dim = int(x.shape[1])
+        codes, scales, middles = self._device_rows(codes, scales, middles, dim)
+        x = _rows_2d(x, "x")
+        kind, out_kind = _dtype_id(x.dtype), _dtype_id(out_dtype or x.dtype)
+        y = torch.empty((x.shape[0], codes.shape[0]), dtype=out_dtype or x.dtype, device=x.device)
+        *p, px, py = _device_pointers(self.dev, codes, scales, middles, x, y)
+        r = self._descriptor(codes, scales, middles, dim, p, _row_stride(codes), _row_stride(scales))
+        self.dev.check(self._lib.vsk_q4_product_dev(self.dev._h, C.byref(r), px, kind, x.shape[0], _row_stride(x), py, out_kind, y.shape[1]))
+        return y
