@@ -572,6 +572,42 @@ int32_t vsk_q4_decode_dev(vsk_ctx* ctx, const vsk_q4_rows* rows, float* out);
 int32_t vsk_q4_product_dev(vsk_ctx* ctx, const vsk_q4_rows* rows, const void* x, int32_t x_dtype, int64_t nq, int64_t x_stride,
                            void* y, int32_t y_dtype, int64_t y_stride);
 
+/* --- a beam search's step --------------------------------------------------------------------
+ * Selection over several rows of scores at once, beside vsk_merge_topk_dev: the k best continuations (beam, token) of
+ * each batch entry, over the logits of an output head or over the scores of the rows that a search found for each
+ * partial chain of retrievals.  With beams = 1 and score 0 it is the top-k of each row.  Device pointers.
+ *   logits      element (b, j, v) at logits[b * batch_stride + j * beam_stride + v]; -inf and NaN are never chosen
+ *   scores      [batch][beams] scores of the partial sequences; a beam whose score is not finite offers nothing
+ *   total       scores[b][j] + logit - log(sum of exp of the row)   normalize != 0; a row of which that sum is zero or
+ *                                                                   not a number (a NaN or +inf in it) offers nothing
+ *               scores[b][j] + logit                                otherwise
+ *               in 64 bits; equal totals are ordered by (beam, token)
+ *   finished    [batch][beams] bytes or NULL: such a beam offers (end_token, at its own score) and nothing else; its
+ *               logits are not read
+ *   out         [batch][k] totals rounded to fp32, descending, with their beams and tokens; places without a candidate have
+ *               score -inf, beam -1, token -1
+ * At most 64 beams, k at most 128, vocabulary and batch below 2^31. */
+int32_t vsk_beam_select_dev(vsk_ctx* ctx, const void* logits, int32_t dtype, int64_t batch, int32_t beams, int64_t vocab,
+                            int64_t batch_stride, int64_t beam_stride, const float* scores, const uint8_t* finished,
+                            int64_t end_token, int32_t normalize, int32_t k, float* out_scores, int64_t* out_beams,
+                            int64_t* out_tokens);
+/* The beams' states (key-value caches, token histories) moved after their parents, all states in one launch or a few:
+ * row (b, i) of dst becomes row (b, parents[b][i]) of src; with parent -1 the row is left as it is.  dst = src (and the
+ * same strides): in place, in any permutation.  Otherwise dst must not overlap any src, and no two states the same
+ * memory.  A row is `outer` parts of steps * step_bytes contiguous bytes.  timed != 0: steps are time steps, and only the
+ * first lengths[b] of them move (lengths NULL: all); the bytes behind are left as they are.
+ * A parent outside [-1, beams) leaves all states of its batch entry as they are and returns VSK_ERR_INVALID_INPUT. */
+typedef struct vsk_state {
+  const void* src;
+  void* dst;
+  int64_t src_row_stride, dst_row_stride;       /* bytes between rows b * beams + i */
+  int64_t src_outer_stride, dst_outer_stride;   /* bytes between the parts of a row */
+  int64_t outer, steps, step_bytes;
+  int32_t timed, reserved;
+} vsk_state;
+int32_t vsk_reorder_states_dev(vsk_ctx* ctx, const vsk_state* states, int32_t count, int64_t batch, int32_t beams,
+                               const int64_t* parents, const int64_t* lengths);
+
 #ifdef __cplusplus
 }
 #endif

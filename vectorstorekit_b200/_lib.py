@@ -55,6 +55,12 @@ class Q4Rows(C.Structure):
                 ("n", C.c_int64), ("dim", C.c_int32), ("group", C.c_int32)]
 
 
+class State(C.Structure):
+    _fields_ = [("src", vp), ("dst", vp), ("src_row_stride", C.c_int64), ("dst_row_stride", C.c_int64), ("src_outer_stride", C.c_int64),
+                ("dst_outer_stride", C.c_int64), ("outer", C.c_int64), ("steps", C.c_int64), ("step_bytes", C.c_int64),
+                ("timed", C.c_int32), ("reserved", C.c_int32)]
+
+
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2   # vsk_dtype
 COMM_ID_BYTES = 128
 SHARDED_SLICE, SHARDED_ALL, SHARDED_QUERIES_SPLIT = 0, 1, 16
@@ -159,6 +165,9 @@ SIGNATURES = {
     "vsk_sq8_index_create": (C.c_int32, [vp, C.c_int32, C.c_int32, vp, vp, C.POINTER(vp)]),
     "vsk_sq8_index_add": (C.c_int32, [vp, vp, C.c_int64]),
     "vsk_sq8_index_add_dev": (C.c_int32, [vp, vp, C.c_int64]),
+    "vsk_beam_select_dev": (C.c_int32, [vp, vp, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_int64, C.c_int64, vp, vp, C.c_int64, C.c_int32,
+                                        C.c_int32, vp, vp, vp]),
+    "vsk_reorder_states_dev": (C.c_int32, [vp, C.POINTER(State), C.c_int32, C.c_int64, C.c_int32, vp, vp]),
     "vsk_q4_encode": (C.c_int32, [vp, vp, C.c_int64, C.c_int32, C.c_int32, C.c_int32, vp, C.c_int64, vp, vp]),
     "vsk_q4_encode_dev": (C.c_int32, [vp, vp, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_int32, C.c_int32, vp, C.c_int64, vp, vp]),
     "vsk_q4_decode": (C.c_int32, [vp, C.POINTER(Q4Rows), vp]),

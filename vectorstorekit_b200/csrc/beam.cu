@@ -1,0 +1,503 @@
+// A beam search's step: the k best (beam, token) continuations of every batch entry, and the beams' states moved after their parents.
+//
+// Selection.  Candidate (j, v) of a live beam j has the total  score_j + (l_jv - lse_j)  (lse_j = log of the sum of exp of row j), or
+// score_j + l_jv without normalisation, in 64 bits; the k largest are wanted, equal totals by the lowest (j, v).  The logits are
+// read once: a warp takes a piece of 1 024 of them and leaves its maximum and its sum of exponentials (running maxima would
+// serialise what a second look at registers does not).  The k best candidates lie in the k pieces with the best maxima, since a piece
+// outside those has k better maxima before every one of its candidates: one block per batch entry ranks the maxima and reads
+// those k pieces again, from L2.
+#include <cuda_bf16.h>
+#include <math_constants.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace vsk {
+namespace {
+
+constexpr int kPiece = 1024;
+constexpr int kMaxBeams = 64;
+constexpr int kMaxBeamK = 128;
+constexpr int kListed = 1024;     // candidates that a selection can order at once
+
+struct BeamArgs {
+  const void* logits;
+  int64_t batch, batch_stride, beam_stride, vocab;
+  int beams, k, normalize;
+  const float* scores;            // [batch][beams]
+  const uint8_t* finished;        // [batch][beams] or null
+  int64_t end_token;
+  float2* stats;                  // [batch * beams][pieces]: maximum, sum of exp(x - maximum)
+  int pieces;
+  float* out_scores;
+  int64_t* out_beams;
+  int64_t* out_tokens;
+};
+
+template <typename T> __device__ __forceinline__ float as_float(T v);
+template <> __device__ __forceinline__ float as_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ float as_float<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float as_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+__device__ __forceinline__ float exp_of(float x) { return exp2f(x * 1.4426950408889634f); }
+
+// ---- one piece per warp -----------------------------------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(256) beam_pieces_kernel(const BeamArgs a) {
+  constexpr int kVec = 16 / sizeof(T), kLoads = kPiece / (32 * kVec);
+  const int lane = threadIdx.x & 31;
+  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t row = item / a.pieces;
+  if (row >= a.batch * a.beams) return;
+  if (!isfinite(__ldg(a.scores + row)) || (a.finished && __ldg(a.finished + row))) return;   // not looked at again
+  const int piece = (int)(item - row * a.pieces);
+  const T* base = reinterpret_cast<const T*>(a.logits) + row / a.beams * a.batch_stride + row % a.beams * a.beam_stride;
+  // pieces begin at 16-byte boundaries of the address, so the first one of a row may begin before it
+  const int64_t first = (int64_t)piece * kPiece - (int64_t)((reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T));
+  float x[kLoads * kVec];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int64_t at = first + (i * 32 + lane) * kVec;
+    if (at >= 0 && at + kVec <= a.vocab) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(base + at));
+      const T* h = reinterpret_cast<const T*>(&v);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) x[i * kVec + j] = as_float<T>(h[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) x[i * kVec + j] = at + j >= 0 && at + j < a.vocab ? as_float<T>(*VSK_CHK(base + at + j)) : -CUDART_INF_F;
+    }
+  }
+  float top = x[0];
+#pragma unroll
+  for (int i = 1; i < kLoads * kVec; ++i) top = fmaxf(top, x[i]);   // (NaN only where all are)
+  if (isnan(top)) top = -CUDART_INF_F;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float sum = 0.f;
+  if (a.normalize) {
+    const float from = top == -CUDART_INF_F ? 0.f : top;   // (+inf stays: its row's sum becomes NaN, and so does a NaN's)
+#pragma unroll
+    for (int i = 0; i < kLoads * kVec; ++i) sum += exp_of(x[i] - from);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  }
+  if (lane == 0) *VSK_CHK_W(a.stats + item) = make_float2(top, sum);
+}
+
+// ---- selection --------------------------------------------------------------------------------------------------------------
+struct Key {
+  double total;
+  int64_t at;
+};
+__device__ __forceinline__ Key no_key() { return Key{-CUDART_INF, 0x7fffffffffffffffLL}; }
+__device__ __forceinline__ bool before(const Key& a, const Key& b) { return a.total > b.total || (a.total == b.total && a.at < b.at); }
+
+// Descending bitonic sort of P = 2^i keys.
+__device__ __forceinline__ void sort_keys(Key* s, int P) {
+  for (int size = 2; size <= P; size <<= 1)
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      for (int i = threadIdx.x; i < (P >> 1); i += blockDim.x) {
+        const int pos = 2 * i - (i & (stride - 1)), other = pos + stride;
+        const Key x = s[pos], y = s[other];
+        if (before(y, x) == ((pos & size) == 0)) {
+          s[pos] = y;
+          s[other] = x;
+        }
+      }
+      __syncthreads();
+    }
+}
+
+// The k best keys of `items`, in order, into list[0 .. return value) (at most k).  key_of(i) may be asked several times.
+// A thread's own best keys are as many as there are threads, so the k-th best of them bounds the k-th best of all from below, and
+// only the k threads with better ones hold keys above it: rarely more than a few times k, and if they are more than the list
+// takes (as many good keys in one thread's share), the best are taken out one by one.
+template <int THREADS, typename F>
+__device__ int best_keys(int64_t items, int k, Key* list, int* count, F key_of) {
+  Key own = no_key();
+  for (int64_t i = threadIdx.x; i < items; i += THREADS) {
+    const Key x = key_of(i);
+    if (before(x, own)) own = x;
+  }
+  list[threadIdx.x] = own;
+  if (threadIdx.x == 0) *count = 0;
+  __syncthreads();
+  sort_keys(list, THREADS);
+  const Key bound = list[k - 1];   // (no_key() where fewer threads have one)
+  __syncthreads();
+  for (int64_t i = threadIdx.x; i < items; i += THREADS) {
+    const Key x = key_of(i);
+    if (x.total > -CUDART_INF && !before(bound, x)) {
+      const int slot = atomicAdd(count, 1);
+      if (slot < kListed) list[slot] = x;
+    }
+  }
+  __syncthreads();
+  const int found = *count;
+  __syncthreads();
+  if (found <= kListed) {
+    int P = 2;
+    while (P < found) P <<= 1;
+    for (int i = found + threadIdx.x; i < P; i += THREADS) list[i] = no_key();
+    __syncthreads();
+    sort_keys(list, P);
+    return min(found, k);
+  }
+  // one by one: the best key behind the last one taken
+  Key last{CUDART_INF, -1};
+  for (int r = 0; r < k; ++r) {
+    own = no_key();
+    for (int64_t i = threadIdx.x; i < items; i += THREADS) {
+      const Key x = key_of(i);
+      if (before(last, x) && before(x, own)) own = x;
+    }
+    Key* room = list + kMaxBeamK;   // (behind the answers)
+    room[threadIdx.x] = own;
+    __syncthreads();
+    for (int o = THREADS / 2; o > 0; o >>= 1) {
+      if (threadIdx.x < o && before(room[threadIdx.x + o], room[threadIdx.x])) room[threadIdx.x] = room[threadIdx.x + o];
+      __syncthreads();
+    }
+    last = room[0];
+    if (threadIdx.x == 0) list[r] = last;
+    __syncthreads();
+  }
+  return k;
+}
+
+// One block per batch entry.  SMALL: the logits themselves are ranked and summed here, without pieces.
+template <typename T, int THREADS, bool SMALL>
+__global__ void __launch_bounds__(THREADS) beam_choose_kernel(const BeamArgs a) {
+  __shared__ Key list[kListed];
+  __shared__ double lse[kMaxBeams], score[kMaxBeams];
+  __shared__ uint8_t kind[kMaxBeams];           // 0: offers nothing, 1: its tokens, 2: finished
+  __shared__ int64_t chosen[kMaxBeamK];
+  __shared__ int count;
+  static_assert(kMaxBeamK + THREADS <= kListed, "best_keys keeps the answers and the threads' keys side by side");
+  const int64_t b = blockIdx.x;
+  const T* base = reinterpret_cast<const T*>(a.logits) + b * a.batch_stride;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  for (int j = warp; j < a.beams; j += THREADS / 32) {
+    const int64_t row = b * a.beams + j;
+    const float s = __ldg(a.scores + row);
+    int what = !isfinite(s) ? 0 : (a.finished && __ldg(a.finished + row)) ? 2 : 1;
+    double total = 0.0;
+    if (what == 1 && a.normalize) {
+      float top = -CUDART_INF_F;
+      double sum = 0.0;
+      if constexpr (SMALL) {
+        for (int v = lane; v < a.vocab; v += 32) top = fmaxf(top, as_float<T>(*VSK_CHK(base + j * a.beam_stride + v)));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        float part = 0.f;
+        if (top > -CUDART_INF_F)
+          for (int v = lane; v < a.vocab; v += 32) part += exp_of(as_float<T>(*VSK_CHK(base + j * a.beam_stride + v)) - top);
+        sum = part;
+      } else {
+        for (int p = lane; p < a.pieces; p += 32) top = fmaxf(top, VSK_CHK(a.stats + row * a.pieces + p)->x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (top > -CUDART_INF_F)
+          for (int p = lane; p < a.pieces; p += 32) {
+            const float2 v = *VSK_CHK(a.stats + row * a.pieces + p);
+            sum += (double)v.y * (double)expf(v.x - top);
+          }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (!(sum > 0.0) || !isfinite(sum)) what = 0;   // nothing but -inf, or a NaN or +inf among the logits
+      else total = (double)top + log(sum);
+    }
+    if (lane == 0) {
+      kind[j] = (uint8_t)what;
+      score[j] = (double)s;
+      lse[j] = total;
+    }
+  }
+  __syncthreads();
+
+  auto total_of = [&](int j, float x) { return score[j] + ((double)x - lse[j]); };   // (lse is 0 without normalisation)
+  auto token_key = [&](int j, int64_t v) {
+    const float x = as_float<T>(*VSK_CHK(base + j * a.beam_stride + v));
+    return x > -CUDART_INF_F ? Key{total_of(j, x), j * a.vocab + v} : no_key();   // (not a NaN either)
+  };
+  int found;
+  if constexpr (SMALL) {
+    const unsigned width = (unsigned)a.vocab;
+    found = best_keys<THREADS>((int64_t)a.beams * a.vocab, a.k, list, &count, [&](int64_t i) {
+      const int j = (int)((unsigned)i / width), v = (int)((unsigned)i % width);
+      if (kind[j] == 1) return token_key(j, v);
+      return kind[j] == 2 && v == 0 ? Key{score[j], j * a.vocab + a.end_token} : no_key();
+    });
+  } else {
+    const unsigned pieces = (unsigned)a.pieces;
+    const int taken = best_keys<THREADS>((int64_t)a.beams * a.pieces, a.k, list, &count, [&](int64_t i) {
+      const int j = (int)((unsigned)i / pieces), p = (int)((unsigned)i % pieces);
+      if (kind[j] == 2) return p == 0 ? Key{score[j], i} : no_key();
+      if (kind[j] == 0) return no_key();
+      const float top = VSK_CHK(a.stats + b * a.beams * a.pieces + i)->x;
+      return top > -CUDART_INF_F ? Key{total_of(j, top), i} : no_key();
+    });
+    if (threadIdx.x < taken) chosen[threadIdx.x] = list[threadIdx.x].at;
+    __syncthreads();
+    found = best_keys<THREADS>((int64_t)taken * kPiece, a.k, list, &count, [&](int64_t i) {
+      const unsigned at = (unsigned)chosen[i / kPiece];
+      const int j = (int)(at / pieces), p = (int)(at % pieces), e = (int)(i % kPiece);
+      if (kind[j] == 2) return e == 0 ? Key{score[j], j * a.vocab + a.end_token} : no_key();
+      const int64_t v = (int64_t)p * kPiece + e - (int64_t)((reinterpret_cast<uintptr_t>(base + j * a.beam_stride) & 15) / sizeof(T));
+      return v >= 0 && v < a.vocab ? token_key(j, v) : no_key();
+    });
+  }
+  for (int r = threadIdx.x; r < a.k; r += THREADS) {
+    const bool has = r < found && list[r].total > -CUDART_INF;
+    const int64_t at = has ? list[r].at : 0;
+    *VSK_CHK_W(a.out_scores + b * a.k + r) = has ? (float)list[r].total : -CUDART_INF_F;
+    *VSK_CHK_W(a.out_beams + b * a.k + r) = has ? at / a.vocab : -1;
+    *VSK_CHK_W(a.out_tokens + b * a.k + r) = has ? at % a.vocab : -1;
+  }
+}
+
+template <typename T>
+int32_t select(Ctx* ctx, BeamArgs a) {
+  // few candidates: one launch without pieces
+  if ((int64_t)a.beams * a.vocab <= 4096) {
+    beam_choose_kernel<T, 128, true><<<(unsigned)a.batch, 128, 0, ctx->stream>>>(a);
+    ctx->stats.kernel_launches++;
+    VSK_CUDA(ctx, cudaGetLastError());
+    return VSK_OK;
+  }
+  a.pieces = (int)ceil_div(a.vocab + 16 / (int)sizeof(T) - 1, kPiece);
+  const int64_t items = a.batch * a.beams * a.pieces, blocks = ceil_div(items, 8);
+  if (blocks > 0x7fffffffLL) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "too many logits in one call");
+  void* p;
+  VSK_TRY(scratch(ctx, SLOT_BEAM, (size_t)items * sizeof(float2), &p));
+  a.stats = (float2*)p;
+  beam_pieces_kernel<T><<<(unsigned)blocks, 256, 0, ctx->stream>>>(a);
+  beam_choose_kernel<T, 512, false><<<(unsigned)a.batch, 512, 0, ctx->stream>>>(a);
+  ctx->stats.kernel_launches += 2;
+  VSK_CUDA(ctx, cudaGetLastError());
+  return VSK_OK;
+}
+
+// ---- states ---------------------------------------------------------------------------------------------------------------------
+// A thread owns one vector of W bytes at one place of all the rows of a batch entry: it loads what every slot takes from its parent and only
+// then stores, so rows may change places in place, in any permutation.
+constexpr int kStatesPerLaunch = 32;
+struct StateMove {
+  const uint8_t* src;
+  uint8_t* dst;
+  int64_t src_row, dst_row, src_outer, dst_outer;   // bytes between rows / between the outer parts of a row
+  int64_t outer, inner;                             // outer parts, bytes of one
+  int64_t step;                                     // bytes of a time step, 0: no time axis
+  int64_t first_block;
+};
+struct StateArgs {
+  StateMove move[kStatesPerLaunch];
+  int count, beams;
+  int64_t batch;
+  const int64_t* parents;     // [batch][beams]
+  const int64_t* lengths;     // [batch] or null
+  int* bad;                   // pinned host memory
+};
+
+template <typename V, int SLOTS>
+__global__ void __launch_bounds__(256) reorder_kernel(const __grid_constant__ StateArgs a) {
+  __shared__ int from[kMaxBeams];
+  __shared__ int moving, wrong;
+  int s = 0;
+  while (s + 1 < a.count && (int64_t)blockIdx.x >= a.move[s + 1].first_block) ++s;
+  const StateMove& m = a.move[s];
+  const int64_t tiles = (m.inner + 256 * sizeof(V) - 1) / (256 * sizeof(V));
+  int64_t at = (int64_t)blockIdx.x - m.first_block;
+  const int64_t tile = at % tiles;
+  at /= tiles;
+  const int64_t part = at % m.outer, b = at / m.outer;
+  int64_t live = m.inner;
+  if (m.step && a.lengths) {
+    const int64_t len = __ldg(a.lengths + b);
+    live = len <= 0 ? 0 : len >= m.inner / m.step ? m.inner : len * m.step;
+  }
+  if (threadIdx.x == 0) moving = wrong = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.beams; i += 256) {
+    const int64_t p = __ldg(a.parents + b * a.beams + i);
+    const bool ok = p >= -1 && p < a.beams;
+    from[i] = ok ? (int)p : -1;
+    if (!ok) wrong = 1;
+    if (ok && p >= 0 && (p != i || m.src != m.dst)) moving = 1;
+  }
+  __syncthreads();
+  if (wrong) {   // every block of this batch entry sees it: none of its rows moves
+    if (threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.bad) = 1;
+    return;
+  }
+  const int64_t off = (tile * 256 + threadIdx.x) * (int64_t)sizeof(V);
+  if (!moving || off >= live) return;
+  const bool here = m.src == m.dst;
+  const uint8_t* src = m.src + b * a.beams * m.src_row + part * m.src_outer + off;
+  uint8_t* dst = m.dst + b * a.beams * m.dst_row + part * m.dst_outer + off;
+  // in place, SLOTS >= beams: everything is loaded before anything is stored
+  for (int i0 = 0; i0 < a.beams; i0 += SLOTS) {
+    V v[SLOTS];
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      const int slot = i0 + i;
+      if (slot < a.beams && from[slot] >= 0 && !(here && from[slot] == slot)) v[i] = *VSK_CHK(reinterpret_cast<const V*>(src + from[slot] * m.src_row));
+    }
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      const int slot = i0 + i;
+      if (slot < a.beams && from[slot] >= 0 && !(here && from[slot] == slot)) *VSK_CHK_W(reinterpret_cast<V*>(dst + slot * m.dst_row)) = v[i];
+    }
+  }
+}
+
+// The largest vector that every address and length of a state is a multiple of.
+int vector_bytes(const vsk_state& s) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(s.src) | reinterpret_cast<uintptr_t>(s.dst) | (uintptr_t)s.src_row_stride |
+                         (uintptr_t)s.dst_row_stride | (s.outer > 1 ? (uintptr_t)(s.src_outer_stride | s.dst_outer_stride) : 0) |
+                         (uintptr_t)s.step_bytes;
+  return (bits & 15) == 0 ? 16 : (bits & 7) == 0 ? 8 : (bits & 3) == 0 ? 4 : (bits & 1) == 0 ? 2 : 1;
+}
+
+template <typename V>
+int32_t reorder(Ctx* ctx, StateArgs& a, bool in_place) {
+  int64_t blocks = 0;
+  for (int i = 0; i < a.count; ++i) {
+    StateMove& m = a.move[i];
+    m.first_block = blocks;
+    blocks += a.batch * m.outer * ceil_div(m.inner, 256 * (int64_t)sizeof(V));
+  }
+  if (blocks > 0x7fffffffLL) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "the states are too large for one call");
+  if (!in_place || a.beams <= 8) reorder_kernel<V, 8><<<(unsigned)blocks, 256, 0, ctx->stream>>>(a);
+  else if (a.beams <= 16) reorder_kernel<V, 16><<<(unsigned)blocks, 256, 0, ctx->stream>>>(a);
+  else if (a.beams <= 32) reorder_kernel<V, 32><<<(unsigned)blocks, 256, 0, ctx->stream>>>(a);
+  else if constexpr (sizeof(V) <= 8) reorder_kernel<V, 64><<<(unsigned)blocks, 256, 0, ctx->stream>>>(a);   // (wider ones come as two)
+  ctx->stats.kernel_launches++;
+  VSK_CUDA(ctx, cudaGetLastError());
+  return VSK_OK;
+}
+
+int32_t check_ctx(vsk_ctx* c, Ctx** ctx) {
+  *ctx = reinterpret_cast<Ctx*>(c);
+  if (!*ctx) return VSK_ERR_INVALID_INPUT;
+  cudaSetDevice((*ctx)->device);
+  return VSK_OK;
+}
+
+}  // namespace
+}  // namespace vsk
+
+using namespace vsk;
+
+extern "C" {
+
+int32_t vsk_beam_select_dev(vsk_ctx* c, const void* logits, int32_t dtype, int64_t batch, int32_t beams, int64_t vocab, int64_t batch_stride,
+                            int64_t beam_stride, const float* scores, const uint8_t* finished, int64_t end_token, int32_t normalize, int32_t k,
+                            float* out_scores, int64_t* out_beams, int64_t* out_tokens) {
+  VSK_TRACE("vsk_beam_select_dev");
+  Ctx* ctx;
+  VSK_TRY(check_ctx(c, &ctx));
+  if (batch <= 0 || beams <= 0 || vocab <= 0) return fail(ctx, VSK_ERR_EMPTY_INPUT, "no candidates");
+  if (beams > kMaxBeams) return fail(ctx, VSK_ERR_INVALID_INPUT, "at most %d beams", kMaxBeams);
+  if (k <= 0 || k > kMaxBeamK) return fail(ctx, VSK_ERR_INVALID_INPUT, "k must be in [1, %d]", kMaxBeamK);
+  if (vocab > 0x7fffffffLL || batch > 0x7fffffffLL) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "vocabulary and batch must be below 2^31");
+  if (!logits || !scores || !out_scores || !out_beams || !out_tokens) return fail(ctx, VSK_ERR_INVALID_INPUT, "null pointer");
+  if (batch_stride < 0 || beam_stride < 0) return fail(ctx, VSK_ERR_INVALID_INPUT, "negative stride");
+  if (finished && (end_token < 0 || end_token >= vocab)) return fail(ctx, VSK_ERR_INVALID_INPUT, "the end token must be in [0, %lld)", (long long)vocab);
+  if (dtype != VSK_DTYPE_F32 && dtype != VSK_DTYPE_F16 && dtype != VSK_DTYPE_BF16)
+    return fail(ctx, VSK_ERR_UNSUPPORTED_OPERATION, "element type %d is not supported", dtype);
+  if (reinterpret_cast<uintptr_t>(logits) & (dtype == VSK_DTYPE_F32 ? 3 : 1)) return fail(ctx, VSK_ERR_INVALID_INPUT, "logits are not aligned to their element");
+  drain_stale_error("vsk_beam_select_dev");
+  BeamArgs a{};
+  a.logits = logits;
+  a.batch = batch;
+  a.batch_stride = batch_stride;
+  a.beam_stride = beam_stride;
+  a.vocab = vocab;
+  a.beams = beams;
+  a.k = k;
+  a.normalize = normalize != 0;
+  a.scores = scores;
+  a.finished = finished;
+  a.end_token = end_token;
+  a.out_scores = out_scores;
+  a.out_beams = out_beams;
+  a.out_tokens = out_tokens;
+  VSK_TRY(dtype == VSK_DTYPE_F32 ? select<float>(ctx, a) : dtype == VSK_DTYPE_F16 ? select<__half>(ctx, a) : select<__nv_bfloat16>(ctx, a));
+  VSK_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+  return VSK_OK;
+}
+
+int32_t vsk_reorder_states_dev(vsk_ctx* c, const vsk_state* states, int32_t count, int64_t batch, int32_t beams, const int64_t* parents,
+                               const int64_t* lengths) {
+  VSK_TRACE("vsk_reorder_states_dev");
+  Ctx* ctx;
+  VSK_TRY(check_ctx(c, &ctx));
+  if (count <= 0 || batch <= 0 || beams <= 0) return fail(ctx, VSK_ERR_EMPTY_INPUT, "no states");
+  if (beams > kMaxBeams) return fail(ctx, VSK_ERR_INVALID_INPUT, "at most %d beams", kMaxBeams);
+  if (batch > 0x7fffffffLL) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "batch must be below 2^31");
+  if (!states || !parents) return fail(ctx, VSK_ERR_INVALID_INPUT, "null pointer");
+  for (int32_t i = 0; i < count; ++i) {
+    const vsk_state& s = states[i];
+    if (!s.src || !s.dst) return fail(ctx, VSK_ERR_INVALID_INPUT, "state %d: null pointer", i);
+    if (s.outer <= 0 || s.steps <= 0 || s.step_bytes <= 0) return fail(ctx, VSK_ERR_EMPTY_INPUT, "state %d is empty", i);
+    if (s.steps > (1ll << 48) / s.step_bytes || s.outer > (1ll << 48) / (s.steps * s.step_bytes))
+      return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "state %d is too large", i);
+    const int64_t inner = s.steps * s.step_bytes;
+    if (s.src_row_stride < 0 || s.src_outer_stride < 0 || s.dst_row_stride < inner || (s.outer > 1 && s.dst_outer_stride < inner))
+      return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "state %d: rows overlap", i);
+    if (s.src == s.dst && (s.src_row_stride != s.dst_row_stride || (s.outer > 1 && s.src_outer_stride != s.dst_outer_stride)))
+      return fail(ctx, VSK_ERR_INVALID_INPUT, "state %d: in place, but with other strides", i);
+    for (int32_t j = 0; j < i; ++j)
+      if (states[j].dst == s.dst || states[j].src == s.dst || s.src == states[j].dst)
+        return fail(ctx, VSK_ERR_INVALID_INPUT, "states %d and %d are the same memory", j, i);
+  }
+  drain_stale_error("vsk_reorder_states_dev");
+  VSK_TRY(pinned_reserve(ctx, &ctx->host_flags[0], sizeof(int)));
+  volatile int* bad = (volatile int*)ctx->host_flags[0].p;
+  *bad = 0;
+  // one launch for the states of one vector width that are moved the same way, up to kStatesPerLaunch
+  for (int width = 16; width >= 1; width >>= 1)
+    for (int in_place = 0; in_place < 2; ++in_place) {
+      StateArgs a{};
+      a.beams = beams;
+      a.batch = batch;
+      a.parents = parents;
+      a.lengths = lengths;
+      a.bad = (int*)ctx->host_flags[0].p;
+      for (int32_t i = 0; i <= count; ++i) {
+        if (i < count) {
+          const vsk_state& s = states[i];
+          int w = vector_bytes(s);
+          if (w == 16 && in_place && beams > 32) w = 8;   // (sixty-four vectors of 16 bytes do not fit the registers)
+          if (w != width || (s.src == s.dst) != (in_place == 1)) continue;
+          StateMove& m = a.move[a.count++];
+          m.src = (const uint8_t*)s.src;
+          m.dst = (uint8_t*)s.dst;
+          m.src_row = s.src_row_stride;
+          m.dst_row = s.dst_row_stride;
+          m.src_outer = s.src_outer_stride;
+          m.dst_outer = s.dst_outer_stride;
+          m.outer = s.outer;
+          m.inner = s.steps * s.step_bytes;
+          m.step = s.timed ? s.step_bytes : 0;
+        }
+        if (a.count == 0 || (i < count && a.count < kStatesPerLaunch)) continue;
+        VSK_TRY(width == 16  ? reorder<uint4>(ctx, a, in_place)
+                : width == 8 ? reorder<uint2>(ctx, a, in_place)
+                : width == 4 ? reorder<uint32_t>(ctx, a, in_place)
+                : width == 2 ? reorder<uint16_t>(ctx, a, in_place)
+                             : reorder<uint8_t>(ctx, a, in_place));
+        a.count = 0;
+      }
+    }
+  VSK_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+  if (*bad) return fail(ctx, VSK_ERR_INVALID_INPUT, "a parent is outside [-1, %d): its batch entry's states were left as they were", beams);
+  return VSK_OK;
+}
+
+}  // extern "C"

@@ -170,6 +170,86 @@ def _ptr(a):
     return C.c_void_p(a.ctypes.data)
 
 
+def _dtype_id(t) -> int:
+    """``vsk_dtype`` of a torch element type."""
+    ids = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+    if t not in ids:
+        raise UnsupportedOperation(f"element type {t} is not supported (float32, float16 or bfloat16)")
+    return ids[t]
+
+
+def _span(t) -> int:
+    """Bytes from a tensor's first element to its last."""
+    if t.numel() == 0:
+        return 0
+    return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _device_pointers(dev: "CUDAComputeDevice", *tensors):
+    """Addresses of CUDA tensors of the device object's GPU (None stays None).  The library works on its own stream: the current
+    torch stream is waited for once, as every call of this package does."""
+    for t in tensors:
+        if t is not None and (not _is_dev(t) or t.device.index != dev.device):
+            raise InvalidInput(f"expected a CUDA tensor on device {dev.device}, got {t.device if hasattr(t, 'device') else type(t).__name__}")
+    torch.cuda.current_stream(dev.device).synchronize()
+    out = []
+    for t in tensors:
+        if t is not None and _lib.CHECKED and t.numel():
+            dev._lib.vsk_checked_register(C.c_void_p(t.data_ptr()), _span(t))
+        out.append(None if t is None else C.c_void_p(t.data_ptr()))
+    return out
+
+
+def _rows_2d(t, what):
+    """A matrix whose rows are contiguous (they may lie inside wider ones); others are copied."""
+    if t.dim() != 2:
+        raise DimensionMismatch(f"{what} must be a matrix, got {t.dim()} dimensions")
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+def _row_stride(t) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _row_parts(t, o, axis):
+    """How a row of a state is laid out: ``outer`` parts of ``steps * per_step`` contiguous elements, in the state and its result.
+    -> (outer, elements of a part, steps, per_step, distance of parts in the state, in the result)"""
+    def contiguous_from(x, d):
+        want = 1
+        for i in range(x.dim() - 1, d - 1, -1):
+            if x.shape[i] > 1 and x.stride(i) != want:
+                return False
+            want *= x.shape[i]
+        return True
+
+    def one_stride(x, first, last):
+        """The distance between places of axes first .. last - 1 taken as one, or None."""
+        sizes = [(x.shape[i], x.stride(i)) for i in range(first, last) if x.shape[i] > 1]
+        for (_, a), (n, c) in zip(sizes, sizes[1:]):
+            if a != n * c:
+                return None
+        return sizes[-1][1] if sizes else 0
+
+    start = axis
+    if start is None:
+        start = next((d for d in range(1, t.dim() + 1) if contiguous_from(t, d) and contiguous_from(o, d)))
+    elif not (contiguous_from(t, start) and contiguous_from(o, start)):
+        raise InvalidInput("a state must be contiguous from its time axis on")
+    a, c = one_stride(t, 1, start), one_stride(o, 1, start)
+    if a is None or c is None:
+        raise InvalidInput("the axes before a state's contiguous part must be evenly spaced")
+    outer = 1
+    for n in t.shape[1:start]:
+        outer *= n
+    inner = 1
+    for n in t.shape[start:]:
+        inner *= n
+    steps = t.shape[axis] if axis is not None else 1
+    return outer, inner, steps, inner // steps, a, c
+
+
 class CUDAComputeDevice:
     """What ``CUDAAcceleratorStrategy.initialize()`` returns: an opened context on one GPU."""
 
@@ -402,6 +482,97 @@ class CUDAAccelerationEngine:
         oi = torch.empty((nq, k), dtype=torch.int64, device=dist.device)
         self.dev.check(self._lib.vsk_merge_topk_dev(self.dev._h, _ptr(dist), _ptr(ids), g, nq, k, _ptr(od), _ptr(oi)))
         return od, oi
+
+    # One step of a beam search.  Beside mergeTopK: a selection over several rows of scores at once, and what has to follow it.
+    def selectBeams(self, logits, scores, k: int, normalize: bool = True, finished=None, end_token: int = 0):
+        """The ``k`` best continuations of every batch entry -> ``(scores, beams, tokens)``, ``[batch][k]`` each, descending, equal
+        totals by the lowest (beam, token).
+
+        ``logits [batch][beams][vocab]`` (float32, float16, bfloat16; any strides before a contiguous last axis) are an output head's,
+        or the scores of the rows that a search found for each chain.  ``scores [batch][beams]`` (float32) are the beams' own.  With
+        ``normalize`` a continuation's total is score + logit - log(sum of exp of its row), without score + logit, in 64 bits.  -inf
+        and NaN are never chosen; a beam whose score is not finite offers nothing.  ``finished [batch][beams]`` (bool): such a
+        beam offers ``end_token`` at its own score and nothing else.  Places without a candidate: -inf, -1, -1.  At most 64 beams, ``k``
+        at most 128.  CUDA tensors; no gradient flows."""
+        if not _is_dev(logits):
+            raise InvalidInput("selectBeams takes CUDA tensors")
+        if logits.dim() != 3:
+            raise DimensionMismatch(f"logits must be [batch][beams][vocab], got {logits.dim()} dimensions")
+        b, w, v = logits.shape
+        kind = _dtype_id(logits.dtype)
+        if b == 0 or w == 0 or v == 0:
+            raise EmptyInput("no candidates")
+        if tuple(scores.shape) != (b, w):
+            raise DimensionMismatch(f"expected scores of shape {(b, w)}, got {tuple(scores.shape)}")
+        if finished is not None and tuple(finished.shape) != (b, w):
+            raise DimensionMismatch(f"expected finished of shape {(b, w)}, got {tuple(finished.shape)}")
+        if not _is_dev(scores) or scores.dtype != torch.float32:
+            raise InvalidInput("scores must be a CUDA tensor of float32")
+        if finished is not None and (not _is_dev(finished) or finished.dtype not in (torch.bool, torch.uint8)):
+            raise InvalidInput("finished must be a CUDA tensor of bool")
+        k = int(k)
+        if not 1 <= k <= 128:
+            raise InvalidInput("k must be in [1, 128]")
+        if v > 1 and logits.stride(2) != 1:
+            logits = logits.contiguous()
+        scores = scores.contiguous()
+        finished = None if finished is None else finished.contiguous()
+        out = torch.empty((b, k), dtype=torch.float32, device=logits.device)
+        beams = torch.empty((b, k), dtype=torch.int64, device=logits.device)
+        tokens = torch.empty((b, k), dtype=torch.int64, device=logits.device)
+        pl, ps, pf, po, pb, pt = _device_pointers(self.dev, logits, scores, finished, out, beams, tokens)
+        self.dev.check(self._lib.vsk_beam_select_dev(self.dev._h, pl, kind, b, w, v, logits.stride(0), logits.stride(1), ps, pf, int(end_token),
+                                                     1 if normalize else 0, k, po, pb, pt))
+        return out, beams, tokens
+
+    def reorderStates(self, states, parents, lengths=None, time_axis=None, out=None):
+        """The beams' states moved after their parents: row ``b * beams + i`` of each result is row ``b * beams + parents[b][i]``.
+
+        ``states``: CUDA tensors ``[batch * beams, ...]`` of any element type (key-value caches, token histories).  ``out=None`` moves
+        them in place, in any permutation; otherwise into the tensors of ``out`` (same shapes and types, other memory).  ``parents
+        [batch][beams]`` int64; a parent of -1 leaves its row as it is.  ``lengths [batch]`` int64 with ``time_axis`` (one number, or one
+        per state; None for a state without time): only the first ``lengths[b]`` places of that axis move, what lies behind stays.
+        At most 64 beams.  Returns ``out``, or ``states``."""
+        states = list(states)
+        if not states:
+            raise EmptyInput("no states")
+        if not _is_dev(parents) or parents.dtype != torch.int64 or parents.dim() != 2:
+            raise InvalidInput("parents must be a CUDA tensor of int64, [batch][beams]")
+        b, w = parents.shape
+        if b == 0 or w == 0:
+            raise EmptyInput("no states")
+        if lengths is not None and (not _is_dev(lengths) or lengths.dtype != torch.int64 or tuple(lengths.shape) != (b,)):
+            raise InvalidInput("lengths must be a CUDA tensor of int64, [batch]")
+        axes = list(time_axis) if isinstance(time_axis, (list, tuple)) else [time_axis] * len(states)
+        results = states if out is None else list(out)
+        if len(axes) != len(states) or len(results) != len(states):
+            raise DimensionMismatch("one time axis and one result per state")
+        moves = (_lib.State * len(states))()
+        for m, t, o, axis in zip(moves, states, results, axes):
+            if not _is_dev(t) or not _is_dev(o):
+                raise InvalidInput("reorderStates takes CUDA tensors")
+            if t.dim() == 0 or t.shape[0] != b * w:
+                raise DimensionMismatch(f"a state must have {b * w} rows, got {tuple(t.shape)}")
+            if o.shape != t.shape or o.dtype != t.dtype:
+                raise DimensionMismatch("a result must have its state's shape and type")
+            if t.numel() == 0:
+                raise EmptyInput("a state is empty")
+            if axis is not None and not 1 <= axis < t.dim():
+                raise InvalidInput(f"time axis {axis} of a state with {t.dim()} dimensions")
+            outer, inner, steps, per_step, src_outer, dst_outer = _row_parts(t, o, axis if lengths is not None else None)
+            e = t.element_size()
+            m.src, m.dst = t.data_ptr(), o.data_ptr()
+            row = inner * outer
+            m.src_row_stride = (t.stride(0) if b * w > 1 else row) * e
+            m.dst_row_stride = (o.stride(0) if b * w > 1 else row) * e
+            m.src_outer_stride, m.dst_outer_stride = src_outer * e, dst_outer * e
+            m.outer, m.steps, m.step_bytes = outer, steps, per_step * e
+            m.timed = 1 if (axis is not None and lengths is not None) else 0
+        parents = parents.contiguous()
+        lengths = None if lengths is None else lengths.contiguous()
+        pp, pl, *_ = _device_pointers(self.dev, parents, lengths, *states, *(results if out is not None else ()))
+        self.dev.check(self._lib.vsk_reorder_states_dev(self.dev._h, moves, len(states), b, w, pp, pl))
+        return results
 
 
 class _IndexBase:

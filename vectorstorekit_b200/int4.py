@@ -10,56 +10,13 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from .engine import (CUDAComputeDevice, DimensionMismatch, EmptyInput, InvalidBufferSize, InvalidInput, UnsupportedOperation, _host,
-                     _is_dev, _ptr)
+from .engine import (CUDAComputeDevice, DimensionMismatch, EmptyInput, InvalidInput, UnsupportedOperation, _device_pointers, _dtype_id,
+                     _host, _is_dev, _ptr, _row_stride, _rows_2d)
 
 try:  # torch is plumbing for device memory only
     import torch
 except Exception:  # pragma: no cover
     torch = None
-
-
-def _dtype_id(t) -> int:
-    """``vsk_dtype`` of a torch element type."""
-    ids = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
-    if t not in ids:
-        raise UnsupportedOperation(f"element type {t} is not supported (float32, float16 or bfloat16)")
-    return ids[t]
-
-
-def _span(t) -> int:
-    """Bytes from a tensor's first element to its last."""
-    if t.numel() == 0:
-        return 0
-    return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-
-
-def _device_pointers(dev: CUDAComputeDevice, *tensors):
-    """Addresses of CUDA tensors of the device object's GPU (None stays None).  The library works on its own stream: the current
-    torch stream is waited for once, as every call of this package does."""
-    for t in tensors:
-        if t is not None and (not _is_dev(t) or t.device.index != dev.device):
-            raise InvalidInput(f"expected a CUDA tensor on device {dev.device}, got {t.device if hasattr(t, 'device') else type(t).__name__}")
-    torch.cuda.current_stream(dev.device).synchronize()
-    out = []
-    for t in tensors:
-        if t is not None and _lib.CHECKED and t.numel():
-            dev._lib.vsk_checked_register(C.c_void_p(t.data_ptr()), _span(t))
-        out.append(None if t is None else C.c_void_p(t.data_ptr()))
-    return out
-
-
-def _rows_2d(t, what):
-    """A matrix whose rows are contiguous (they may lie inside wider ones); others are copied."""
-    if t.dim() != 2:
-        raise DimensionMismatch(f"{what} must be a matrix, got {t.dim()} dimensions")
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
-    return t
-
-
-def _row_stride(t) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
 
 
 class Int4Quantizer:
