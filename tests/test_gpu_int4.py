@@ -259,6 +259,7 @@ def test_int4_refusals(dev):
     from vectorstorekit_b200 import _lib
     p = lambda t: C.c_void_p(t.data_ptr())
     y = torch.empty((4, 4), device="cuda")
+    lib.vsk_checked_register(p(y), 64)
     r = _lib.Q4Rows(p(codes), p(scales), None, 32, 2, 4, 64, 32)
 
     def product(**kw):

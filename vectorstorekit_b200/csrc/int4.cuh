@@ -8,4 +8,8 @@ namespace vsk {
 int32_t q4_product(Ctx* ctx, const vsk_q4_rows& rows, const void* x, int32_t x_dtype, int64_t nq, int64_t x_stride, void* y,
                    int32_t y_dtype, int64_t y_stride);
 
+// The same in whole numbers, for a few vectors (int4_digits.cu).
+int32_t q4_product_digits(Ctx* ctx, const vsk_q4_rows& rows, const void* x, int32_t x_dtype, int64_t nq, int64_t x_stride, void* y,
+                          int32_t y_dtype, int64_t y_stride);
+
 }  // namespace vsk
