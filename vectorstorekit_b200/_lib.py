@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 # VSK_CHECKED=1 selects the checked build variant (the kernels' read-only loads and atomics range-tested; see
@@ -55,11 +56,7 @@ class Q4Rows(C.Structure):
                 ("n", C.c_int64), ("dim", C.c_int32), ("group", C.c_int32)]
 
 
-class State(C.Structure):
-    _fields_ = [("src", vp), ("dst", vp), ("src_row_stride", C.c_int64), ("dst_row_stride", C.c_int64), ("src_outer_stride", C.c_int64),
-                ("dst_outer_stride", C.c_int64), ("outer", C.c_int64), ("steps", C.c_int64), ("step_bytes", C.c_int64),
-                ("timed", C.c_int32), ("reserved", C.c_int32)]
-
+STATE = struct.Struct("2P7q2i")   # vsk_state, as a list of them is packed
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2   # vsk_dtype
 COMM_ID_BYTES = 128
@@ -167,7 +164,7 @@ SIGNATURES = {
     "vsk_sq8_index_add_dev": (C.c_int32, [vp, vp, C.c_int64]),
     "vsk_beam_select_dev": (C.c_int32, [vp, vp, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_int64, C.c_int64, vp, vp, C.c_int64, C.c_int32,
                                         C.c_int32, vp, vp, vp]),
-    "vsk_reorder_states_dev": (C.c_int32, [vp, C.POINTER(State), C.c_int32, C.c_int64, C.c_int32, vp, vp]),
+    "vsk_reorder_states_dev": (C.c_int32, [vp, vp, C.c_int32, C.c_int64, C.c_int32, vp, vp]),
     "vsk_q4_encode": (C.c_int32, [vp, vp, C.c_int64, C.c_int32, C.c_int32, C.c_int32, vp, C.c_int64, vp, vp]),
     "vsk_q4_encode_dev": (C.c_int32, [vp, vp, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_int32, C.c_int32, vp, C.c_int64, vp, vp]),
     "vsk_q4_decode": (C.c_int32, [vp, C.POINTER(Q4Rows), vp]),

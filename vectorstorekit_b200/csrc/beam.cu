@@ -2,10 +2,11 @@
 //
 // Selection.  Candidate (j, v) of a live beam j has the total  score_j + (l_jv - lse_j)  (lse_j = log of the sum of exp of row j), or
 // score_j + l_jv without normalisation, in 64 bits; the k largest are wanted, equal totals by the lowest (j, v).  The logits are
-// read once: a warp takes a piece of 1 024 of them and leaves its maximum and its sum of exponentials (running maxima would
-// serialise what a second look at registers does not).  The k best candidates lie in the k pieces with the best maxima, since a piece
-// outside those has k better maxima before every one of its candidates: one block per batch entry ranks the maxima and reads
-// those k pieces again, from L2.
+// read once: a warp takes a piece of 1 024 of them and leaves its maximum and its sum of exponentials (a second look at registers
+// instead of running maxima).  The k best candidates lie in the k pieces with the best maxima, since a piece outside those has k
+// better maxima before every one of its candidates: one block per batch entry finds a bound that at least k pieces reach and reads
+// those pieces again, from L2, for the candidates that reach it too.  Few candidates are staged in shared memory instead and need
+// no pieces.
 #include <cuda_bf16.h>
 #include <math_constants.h>
 
@@ -20,39 +21,55 @@ constexpr int kPiece = 1024;
 constexpr int kMaxBeams = 64;
 constexpr int kMaxBeamK = 128;
 constexpr int kListed = 1024;     // candidates that a selection can order at once
+constexpr int kChosen = 512;      // pieces that it reads again
+constexpr int kSmall = 8192;      // candidates of a batch entry that are staged in shared memory
 
 struct BeamArgs {
   const void* logits;
   int64_t batch, batch_stride, beam_stride, vocab;
+  int64_t first_batch;            // of a launch of beam_pieces_kernel
   int beams, k, normalize;
   const float* scores;            // [batch][beams]
   const uint8_t* finished;        // [batch][beams] or null
   int64_t end_token;
   float2* stats;                  // [batch * beams][pieces]: maximum, sum of exp(x - maximum)
+  float* parts;                   // [batch * beams][pieces][parts of one]: maxima of what one load of a warp brings, or null
   int pieces;
   float* out_scores;
   int64_t* out_beams;
   int64_t* out_tokens;
 };
 
+__device__ __forceinline__ void wait_for_launches_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_the_next_launch_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 template <typename T> __device__ __forceinline__ float as_float(T v);
 template <> __device__ __forceinline__ float as_float<float>(float v) { return v; }
 template <> __device__ __forceinline__ float as_float<__half>(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float as_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-__device__ __forceinline__ float exp_of(float x) { return exp2f(x * 1.4426950408889634f); }
+// (x - from) first: it is exact near the maximum, however large the logits are.
+__device__ __forceinline__ float exp_of(float x, float from) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"((x - from) * 1.4426950408889634f));
+  return r;
+}
+__device__ __forceinline__ float reference_of(float top) { return top == -CUDART_INF_F ? 0.f : top; }
+
+__device__ __forceinline__ float warp_max(float x) { return ordered_to_float(__reduce_max_sync(0xffffffffu, float_to_ordered(x))); }
 
 // ---- one piece per warp -----------------------------------------------------------------------------------------------------
+// 32 x 8 x 131 072 bf16 logits (67 MB): bound by the instructions of a logit (convert, maximum, subtract, multiply, power, add).
 template <typename T>
 __global__ void __launch_bounds__(256) beam_pieces_kernel(const BeamArgs a) {
   constexpr int kVec = 16 / sizeof(T), kLoads = kPiece / (32 * kVec);
+  let_the_next_launch_begin();
   const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int64_t row = item / a.pieces;
-  if (row >= a.batch * a.beams) return;
+  const int piece = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (piece >= a.pieces) return;
+  const int64_t b = a.first_batch + blockIdx.z, row = b * a.beams + blockIdx.y, item = row * a.pieces + piece;
   if (!isfinite(__ldg(a.scores + row)) || (a.finished && __ldg(a.finished + row))) return;   // not looked at again
-  const int piece = (int)(item - row * a.pieces);
-  const T* base = reinterpret_cast<const T*>(a.logits) + row / a.beams * a.batch_stride + row % a.beams * a.beam_stride;
+  const T* base = reinterpret_cast<const T*>(a.logits) + b * a.batch_stride + blockIdx.y * a.beam_stride;
   // pieces begin at 16-byte boundaries of the address, so the first one of a row may begin before it
   const int64_t first = (int64_t)piece * kPiece - (int64_t)((reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T));
   float x[kLoads * kVec];
@@ -69,17 +86,27 @@ __global__ void __launch_bounds__(256) beam_pieces_kernel(const BeamArgs a) {
       for (int j = 0; j < kVec; ++j) x[i * kVec + j] = at + j >= 0 && at + j < a.vocab ? as_float<T>(*VSK_CHK(base + at + j)) : -CUDART_INF_F;
     }
   }
-  float top = x[0];
+  float own[kLoads], top = -CUDART_INF_F;
 #pragma unroll
-  for (int i = 1; i < kLoads * kVec; ++i) top = fmaxf(top, x[i]);   // (NaN only where all are)
-  if (isnan(top)) top = -CUDART_INF_F;
+  for (int i = 0; i < kLoads; ++i) {
+    own[i] = -CUDART_INF_F;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int j = 0; j < kVec; ++j) own[i] = fmaxf(own[i], x[i * kVec + j]);   // (a NaN is passed over)
+    top = fmaxf(top, own[i]);
+  }
+  top = warp_max(top);
+  if (a.parts) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const float m = warp_max(own[i]);
+      if (lane == i) *VSK_CHK_W(a.parts + item * kLoads + i) = m;
+    }
+  }
   float sum = 0.f;
   if (a.normalize) {
-    const float from = top == -CUDART_INF_F ? 0.f : top;   // (+inf stays: its row's sum becomes NaN, and so does a NaN's)
+    const float from = reference_of(top);   // (+inf stays: its row's sum becomes NaN, and so does a NaN's)
 #pragma unroll
-    for (int i = 0; i < kLoads * kVec; ++i) sum += exp_of(x[i] - from);
+    for (int i = 0; i < kLoads * kVec; ++i) sum += exp_of(x[i], from);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
@@ -167,19 +194,60 @@ __device__ int best_keys(int64_t items, int k, Key* list, int* count, F key_of) 
   return k;
 }
 
-// One block per batch entry.  SMALL: the logits themselves are ranked and summed here, without pieces.
+// The largest bound that at least k threads' keys reach, or nearly the largest (at most half as many again do, if the keys differ enough);
+// 1 where fewer than k threads have one.  Keys are the order of fp32 numbers, 0: none.
+template <int THREADS>
+__device__ unsigned bound_of(unsigned own, int k, unsigned* shared) {
+  if (threadIdx.x == 0) {
+    shared[0] = 0xffffffffu;
+    shared[1] = 0u;
+  }
+  const int real = __syncthreads_count(own != 0u);
+  if (real <= k) return 1u;
+  const unsigned low = __reduce_min_sync(0xffffffffu, own ? own : 0xffffffffu), high = __reduce_max_sync(0xffffffffu, own);
+  if ((threadIdx.x & 31) == 0) {
+    atomicMin(&shared[0], low);
+    atomicMax(&shared[1], high);
+  }
+  __syncthreads();
+  unsigned lo = shared[0], hi = shared[1];   // at least k reach lo; hi may be too much
+  while (lo < hi) {
+    const unsigned mid = lo + (hi - lo + 1) / 2;
+    const int reach = __syncthreads_count(own >= mid);
+    if (reach >= k) {
+      lo = mid;
+      if (reach <= k + k / 2) break;
+    } else {
+      hi = mid - 1;
+    }
+  }
+  return lo;
+}
+
+// One block per batch entry.  SMALL: the candidates are staged in shared memory; otherwise their pieces are ranked first.
 template <typename T, int THREADS, bool SMALL>
 __global__ void __launch_bounds__(THREADS) beam_choose_kernel(const BeamArgs a) {
   __shared__ Key list[kListed];
   __shared__ double lse[kMaxBeams], score[kMaxBeams];
   __shared__ uint8_t kind[kMaxBeams];           // 0: offers nothing, 1: its tokens, 2: finished
   __shared__ int64_t chosen[kMaxBeamK];
-  __shared__ int count;
+  __shared__ int piece_list[SMALL ? 1 : kChosen];
+  __shared__ int count, taken_pieces;
+  __shared__ unsigned range[2];
+  extern __shared__ float staged[];             // SMALL: [beams][vocab]
   static_assert(kMaxBeamK + THREADS <= kListed, "best_keys keeps the answers and the threads' keys side by side");
+  static_assert(THREADS >= kMaxBeamK, "the k-th best of the threads' keys");
   const int64_t b = blockIdx.x;
   const T* base = reinterpret_cast<const T*>(a.logits) + b * a.batch_stride;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned width = (unsigned)a.vocab;
 
+  if constexpr (!SMALL) wait_for_launches_before();   // the pieces
+  if constexpr (SMALL) {
+    for (int j = 0; j < a.beams; ++j)
+      for (unsigned v = threadIdx.x; v < width; v += THREADS) staged[j * width + v] = as_float<T>(*VSK_CHK(base + j * a.beam_stride + v));
+    __syncthreads();
+  }
   for (int j = warp; j < a.beams; j += THREADS / 32) {
     const int64_t row = b * a.beams + j;
     const float s = __ldg(a.scores + row);
@@ -189,22 +257,27 @@ __global__ void __launch_bounds__(THREADS) beam_choose_kernel(const BeamArgs a) 
       float top = -CUDART_INF_F;
       double sum = 0.0;
       if constexpr (SMALL) {
-        for (int v = lane; v < a.vocab; v += 32) top = fmaxf(top, as_float<T>(*VSK_CHK(base + j * a.beam_stride + v)));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (unsigned v = lane; v < width; v += 32) top = fmaxf(top, staged[j * width + v]);
+        top = warp_max(top);
+        const float from = reference_of(top);
         float part = 0.f;
-        if (top > -CUDART_INF_F)
-          for (int v = lane; v < a.vocab; v += 32) part += exp_of(as_float<T>(*VSK_CHK(base + j * a.beam_stride + v)) - top);
+        for (unsigned v = lane; v < width; v += 32) part += exp_of(staged[j * width + v], from);
         sum = part;
       } else {
-        for (int p = lane; p < a.pieces; p += 32) top = fmaxf(top, VSK_CHK(a.stats + row * a.pieces + p)->x);
+        const float2* stats = a.stats + row * a.pieces;
+        float2 held[4];   // the first 128 pieces' are read once
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (top > -CUDART_INF_F)
-          for (int p = lane; p < a.pieces; p += 32) {
-            const float2 v = *VSK_CHK(a.stats + row * a.pieces + p);
-            sum += (double)v.y * (double)expf(v.x - top);
-          }
+        for (int i = 0; i < 4; ++i) held[i] = lane + 32 * i < a.pieces ? *VSK_CHK(stats + lane + 32 * i) : make_float2(-CUDART_INF_F, 0.f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, held[i].x);
+        for (int p = lane + 128; p < a.pieces; p += 32) top = fmaxf(top, VSK_CHK(stats + p)->x);
+        top = warp_max(top);
+        const float from = reference_of(top);
+        // (a piece of nothing but -inf and NaN: its sum is 0 or NaN)
+        auto share = [&](const float2& v) { sum += v.x == -CUDART_INF_F ? (double)v.y : (double)v.y * (double)exp_of(v.x, from); };
+#pragma unroll
+        for (int i = 0; i < 4; ++i) share(held[i]);
+        for (int p = lane + 128; p < a.pieces; p += 32) share(*VSK_CHK(stats + p));
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -217,28 +290,134 @@ __global__ void __launch_bounds__(THREADS) beam_choose_kernel(const BeamArgs a) 
       lse[j] = total;
     }
   }
+  if (threadIdx.x == 0) count = taken_pieces = 0;
   __syncthreads();
 
   auto total_of = [&](int j, float x) { return score[j] + ((double)x - lse[j]); };   // (lse is 0 without normalisation)
-  auto token_key = [&](int j, int64_t v) {
-    const float x = as_float<T>(*VSK_CHK(base + j * a.beam_stride + v));
-    return x > -CUDART_INF_F ? Key{total_of(j, x), j * a.vocab + v} : no_key();   // (not a NaN either)
+  // the order of a total as fp32, 0: no candidate.  (Rounding keeps the order, up to equality.)
+  auto order_of = [&](int j, float x) -> unsigned { return x > -CUDART_INF_F ? float_to_ordered((float)total_of(j, x) + 0.f) : 0u; };   // (not a NaN either)
+  auto token_key = [&](int j, int64_t v, float x) { return x > -CUDART_INF_F ? Key{total_of(j, x), j * a.vocab + v} : no_key(); };
+  auto add = [&](const Key& x) {
+    const int slot = atomicAdd(&count, 1);
+    if (slot < kListed) list[slot] = x;
   };
-  int found;
+  const unsigned pieces = (unsigned)a.pieces;
+  constexpr int kVec = 16 / sizeof(T), kParts = kPiece / (32 * kVec);
+  const unsigned per_piece = !SMALL && a.parts ? kParts : 1;
+  // part i of the pieces (all parts, or whole pieces)
+  auto part_order = [&](unsigned i) -> unsigned {
+    const unsigned at = i / per_piece, j = at / pieces;
+    if (kind[j] == 2) return i % (per_piece * pieces) == 0 ? float_to_ordered((float)score[j] + 0.f) : 0u;
+    if (kind[j] == 0) return 0u;
+    const int64_t of = b * a.beams * pieces;
+    return order_of(j, a.parts ? *VSK_CHK(a.parts + of * kParts + i) : VSK_CHK(a.stats + of + i)->x);
+  };
+
+  // A bound that at least k candidates reach; those that do.
+  bool fits = true;
   if constexpr (SMALL) {
-    const unsigned width = (unsigned)a.vocab;
-    found = best_keys<THREADS>((int64_t)a.beams * a.vocab, a.k, list, &count, [&](int64_t i) {
-      const int j = (int)((unsigned)i / width), v = (int)((unsigned)i % width);
-      if (kind[j] == 1) return token_key(j, v);
+    const unsigned items = (unsigned)a.beams * width;
+    auto element = [&](unsigned i) -> unsigned {
+      const unsigned j = i / width;
+      if (kind[j] == 1) return order_of(j, staged[i]);
+      return kind[j] == 2 && i % width == 0 ? float_to_ordered((float)score[j] + 0.f) : 0u;
+    };
+    unsigned own = 0u;
+    for (unsigned i = threadIdx.x; i < items; i += THREADS) own = max(own, element(i));
+    const unsigned bound = bound_of<THREADS>(own, a.k, range);
+    if (own >= bound)
+      for (unsigned i = threadIdx.x; i < items; i += THREADS)
+        if (element(i) >= bound) {
+          const unsigned j = i / width;
+          add(kind[j] == 2 ? Key{score[j], j * a.vocab + a.end_token} : token_key(j, i % width, staged[i]));
+        }
+  } else {
+    const unsigned items = (unsigned)a.beams * pieces * per_piece;
+    unsigned own = 0u;
+#pragma unroll 4
+    for (unsigned i = threadIdx.x; i < items; i += THREADS) own = max(own, part_order(i));
+    const unsigned bound = bound_of<THREADS>(own, a.k, range);
+    if (own >= bound)
+      for (unsigned i = threadIdx.x; i < items; i += THREADS)
+        if (items <= THREADS || part_order(i) >= bound) {
+          const int slot = atomicAdd(&taken_pieces, 1);
+          if (slot < kChosen) piece_list[slot] = (int)i;
+        }
+    __syncthreads();
+    fits = taken_pieces <= kChosen;
+    if (fits) {
+      // a warp per part: what one of its loads brings, or all loads of a whole piece
+      for (int s = warp; s < taken_pieces; s += THREADS / 32) {
+        const unsigned i = (unsigned)piece_list[s], at = i / per_piece, j = at / pieces;
+        if (kind[j] == 2) {
+          if (lane == 0) add(Key{score[j], j * a.vocab + a.end_token});
+          continue;
+        }
+        const T* row = base + j * a.beam_stride;
+        const int64_t first = (int64_t)(at % pieces) * kPiece - (int64_t)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+        const int l0 = a.parts ? (int)(i % per_piece) : 0, l1 = a.parts ? l0 + 1 : kParts;
+#pragma unroll 4
+        for (int l = l0; l < l1; ++l) {
+          const int64_t v0 = first + (l * 32 + lane) * kVec;
+          float x[kVec];
+          if (v0 >= 0 && v0 + kVec <= a.vocab) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + v0));
+            const T* h = reinterpret_cast<const T*>(&u);
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) x[e] = as_float<T>(h[e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) x[e] = v0 + e >= 0 && v0 + e < a.vocab ? as_float<T>(*VSK_CHK(row + v0 + e)) : -CUDART_INF_F;
+          }
+          float top = x[0];
+#pragma unroll
+          for (int e = 1; e < kVec; ++e) top = fmaxf(top, x[e]);
+          if (top > -CUDART_INF_F && order_of(j, top) >= bound) {
+#pragma unroll
+            for (int e = 0; e < kVec; ++e)
+              if (order_of(j, x[e]) >= bound) add(token_key(j, v0 + e, x[e]));
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int reach = count;
+
+  auto put = [&](int r, const Key& x) {
+    const bool has = x.total > -CUDART_INF;
+    *VSK_CHK_W(a.out_scores + b * a.k + r) = has ? (float)x.total : -CUDART_INF_F;
+    *VSK_CHK_W(a.out_beams + b * a.k + r) = has ? x.at / a.vocab : -1;
+    *VSK_CHK_W(a.out_tokens + b * a.k + r) = has ? x.at % a.vocab : -1;
+  };
+  if (fits && reach <= kListed) {
+    // a candidate's place is the number of those before it
+    for (int i = threadIdx.x; i < reach; i += THREADS) {
+      const Key x = list[i];
+      int place = 0;
+      for (int j = 0; j < reach; ++j) place += before(list[j], x);
+      if (place < a.k) put(place, x);
+    }
+    for (int r = reach + threadIdx.x; r < a.k; r += THREADS) put(r, no_key());
+    return;
+  }
+
+  // Many equal totals, or many candidates in few places: exact keys throughout.
+  int found;
+  __syncthreads();
+  if constexpr (SMALL) {
+    found = best_keys<THREADS>((int64_t)a.beams * width, a.k, list, &count, [&](int64_t i) {
+      const int j = (int)((unsigned)i / width);
+      const unsigned v = (unsigned)i % width;
+      if (kind[j] == 1) return token_key(j, v, staged[i]);
       return kind[j] == 2 && v == 0 ? Key{score[j], j * a.vocab + a.end_token} : no_key();
     });
   } else {
-    const unsigned pieces = (unsigned)a.pieces;
-    const int taken = best_keys<THREADS>((int64_t)a.beams * a.pieces, a.k, list, &count, [&](int64_t i) {
+    const int taken = best_keys<THREADS>((int64_t)a.beams * pieces, a.k, list, &count, [&](int64_t i) {
       const int j = (int)((unsigned)i / pieces), p = (int)((unsigned)i % pieces);
       if (kind[j] == 2) return p == 0 ? Key{score[j], i} : no_key();
       if (kind[j] == 0) return no_key();
-      const float top = VSK_CHK(a.stats + b * a.beams * a.pieces + i)->x;
+      const float top = VSK_CHK(a.stats + b * a.beams * pieces + i)->x;
       return top > -CUDART_INF_F ? Key{total_of(j, top), i} : no_key();
     });
     if (threadIdx.x < taken) chosen[threadIdx.x] = list[threadIdx.x].at;
@@ -248,36 +427,54 @@ __global__ void __launch_bounds__(THREADS) beam_choose_kernel(const BeamArgs a) 
       const int j = (int)(at / pieces), p = (int)(at % pieces), e = (int)(i % kPiece);
       if (kind[j] == 2) return e == 0 ? Key{score[j], j * a.vocab + a.end_token} : no_key();
       const int64_t v = (int64_t)p * kPiece + e - (int64_t)((reinterpret_cast<uintptr_t>(base + j * a.beam_stride) & 15) / sizeof(T));
-      return v >= 0 && v < a.vocab ? token_key(j, v) : no_key();
+      return v >= 0 && v < a.vocab ? token_key(j, v, as_float<T>(*VSK_CHK(base + j * a.beam_stride + v))) : no_key();
     });
   }
-  for (int r = threadIdx.x; r < a.k; r += THREADS) {
-    const bool has = r < found && list[r].total > -CUDART_INF;
-    const int64_t at = has ? list[r].at : 0;
-    *VSK_CHK_W(a.out_scores + b * a.k + r) = has ? (float)list[r].total : -CUDART_INF_F;
-    *VSK_CHK_W(a.out_beams + b * a.k + r) = has ? at / a.vocab : -1;
-    *VSK_CHK_W(a.out_tokens + b * a.k + r) = has ? at % a.vocab : -1;
-  }
+  for (int r = threadIdx.x; r < a.k; r += THREADS) put(r, r < found ? list[r] : no_key());
 }
 
 template <typename T>
 int32_t select(Ctx* ctx, BeamArgs a) {
-  // few candidates: one launch without pieces
-  if ((int64_t)a.beams * a.vocab <= 4096) {
-    beam_choose_kernel<T, 128, true><<<(unsigned)a.batch, 128, 0, ctx->stream>>>(a);
+  const int64_t candidates = a.beams * a.vocab;
+  if (candidates <= kSmall) {
+    const size_t shared = (size_t)candidates * sizeof(float);
+    if (candidates <= 2048) beam_choose_kernel<T, 128, true><<<(unsigned)a.batch, 128, shared, ctx->stream>>>(a);
+    else {
+      // (the list and the candidates together pass 48 KB)
+      VSK_CUDA(ctx, opt_in_shared(ctx, beam_choose_kernel<T, 512, true>, kSmall * sizeof(float)));
+      beam_choose_kernel<T, 512, true><<<(unsigned)a.batch, 512, shared, ctx->stream>>>(a);
+    }
     ctx->stats.kernel_launches++;
     VSK_CUDA(ctx, cudaGetLastError());
     return VSK_OK;
   }
+  constexpr int kParts = kPiece * (int)sizeof(T) / 512;
   a.pieces = (int)ceil_div(a.vocab + 16 / (int)sizeof(T) - 1, kPiece);
-  const int64_t items = a.batch * a.beams * a.pieces, blocks = ceil_div(items, 8);
-  if (blocks > 0x7fffffffLL) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "too many logits in one call");
+  const int64_t items = a.batch * a.beams * a.pieces;
+  // parts of pieces where whole ones are few against k: the bound then leaves fewer candidates
+  const bool parts = (int64_t)a.beams * a.pieces < 16 * (int64_t)a.k;
   void* p;
-  VSK_TRY(scratch(ctx, SLOT_BEAM, (size_t)items * sizeof(float2), &p));
+  VSK_TRY(scratch(ctx, SLOT_BEAM, (size_t)items * (sizeof(float2) + (parts ? kParts * sizeof(float) : 0)), &p));
   a.stats = (float2*)p;
-  beam_pieces_kernel<T><<<(unsigned)blocks, 256, 0, ctx->stream>>>(a);
-  beam_choose_kernel<T, 512, false><<<(unsigned)a.batch, 512, 0, ctx->stream>>>(a);
-  ctx->stats.kernel_launches += 2;
+  a.parts = parts ? (float*)(a.stats + items) : nullptr;
+  for (int64_t f = 0; f < a.batch; f += 65535) {
+    a.first_batch = f;
+    beam_pieces_kernel<T><<<dim3((unsigned)ceil_div(a.pieces, 8), (unsigned)a.beams, (unsigned)std::min<int64_t>(65535, a.batch - f)), 256, 0,
+                           ctx->stream>>>(a);
+    ctx->stats.kernel_launches++;
+    VSK_CUDA(ctx, cudaGetLastError());
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)a.batch);
+  cfg.blockDim = dim3(512);
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  VSK_CUDA(ctx, cudaLaunchKernelEx(&cfg, beam_choose_kernel<T, 512, false>, a));
+  ctx->stats.kernel_launches++;
   VSK_CUDA(ctx, cudaGetLastError());
   return VSK_OK;
 }

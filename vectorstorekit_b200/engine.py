@@ -170,12 +170,15 @@ def _ptr(a):
     return C.c_void_p(a.ctypes.data)
 
 
+_DTYPE_IDS = {} if torch is None else {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+
+
 def _dtype_id(t) -> int:
     """``vsk_dtype`` of a torch element type."""
-    ids = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
-    if t not in ids:
+    kind = _DTYPE_IDS.get(t)
+    if kind is None:
         raise UnsupportedOperation(f"element type {t} is not supported (float32, float16 or bfloat16)")
-    return ids[t]
+    return kind
 
 
 def _span(t) -> int:
@@ -188,23 +191,26 @@ def _span(t) -> int:
 def _device_pointers(dev: "CUDAComputeDevice", *tensors):
     """Addresses of CUDA tensors of the device object's GPU (None stays None).  The library works on its own stream: the current
     torch stream is waited for once, as every call of this package does."""
+    index = dev.device
     for t in tensors:
-        if t is not None and (not _is_dev(t) or t.device.index != dev.device):
-            raise InvalidInput(f"expected a CUDA tensor on device {dev.device}, got {t.device if hasattr(t, 'device') else type(t).__name__}")
-    torch.cuda.current_stream(dev.device).synchronize()
-    out = []
-    for t in tensors:
-        if t is not None and _lib.CHECKED and t.numel():
-            dev._lib.vsk_checked_register(C.c_void_p(t.data_ptr()), _span(t))
-        out.append(None if t is None else C.c_void_p(t.data_ptr()))
-    return out
+        if t is not None and t.get_device() != index:
+            raise InvalidInput(f"expected a CUDA tensor on device {index}, got one on {t.device}")
+    torch.cuda.current_stream(index).synchronize()
+    if _lib.CHECKED:
+        for t in tensors:
+            if t is not None and t.numel():
+                dev._lib.vsk_checked_register(C.c_void_p(t.data_ptr()), _span(t))
+    return [None if t is None else t.data_ptr() for t in tensors]
 
 
 def _rows_2d(t, what):
     """A matrix whose rows are contiguous (they may lie inside wider ones); others are copied."""
     if t.dim() != 2:
         raise DimensionMismatch(f"{what} must be a matrix, got {t.dim()} dimensions")
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    if t.is_contiguous():
+        return t
+    (rows, columns), (per_row, step) = t.shape, t.stride()
+    if (columns > 1 and step != 1) or (rows > 1 and per_row < columns):
         t = t.contiguous()
     return t
 
@@ -502,9 +508,9 @@ class CUDAAccelerationEngine:
         kind = _dtype_id(logits.dtype)
         if b == 0 or w == 0 or v == 0:
             raise EmptyInput("no candidates")
-        if tuple(scores.shape) != (b, w):
+        if scores.shape != (b, w):
             raise DimensionMismatch(f"expected scores of shape {(b, w)}, got {tuple(scores.shape)}")
-        if finished is not None and tuple(finished.shape) != (b, w):
+        if finished is not None and finished.shape != (b, w):
             raise DimensionMismatch(f"expected finished of shape {(b, w)}, got {tuple(finished.shape)}")
         if not _is_dev(scores) or scores.dtype != torch.float32:
             raise InvalidInput("scores must be a CUDA tensor of float32")
@@ -513,16 +519,18 @@ class CUDAAccelerationEngine:
         k = int(k)
         if not 1 <= k <= 128:
             raise InvalidInput("k must be in [1, 128]")
-        if v > 1 and logits.stride(2) != 1:
+        per_batch, per_beam, step = logits.stride()
+        if v > 1 and step != 1:
             logits = logits.contiguous()
+            per_batch, per_beam = w * v, v
         scores = scores.contiguous()
         finished = None if finished is None else finished.contiguous()
-        out = torch.empty((b, k), dtype=torch.float32, device=logits.device)
-        beams = torch.empty((b, k), dtype=torch.int64, device=logits.device)
-        tokens = torch.empty((b, k), dtype=torch.int64, device=logits.device)
-        pl, ps, pf, po, pb, pt = _device_pointers(self.dev, logits, scores, finished, out, beams, tokens)
-        self.dev.check(self._lib.vsk_beam_select_dev(self.dev._h, pl, kind, b, w, v, logits.stride(0), logits.stride(1), ps, pf, int(end_token),
-                                                     1 if normalize else 0, k, po, pb, pt))
+        out = scores.new_empty((b, k))
+        places = torch.empty((2, b, k), dtype=torch.int64, device=logits.device)
+        beams, tokens = places.unbind(0)
+        pl, ps, pf, po, pp = _device_pointers(self.dev, logits, scores, finished, out, places)
+        self.dev.check(self._lib.vsk_beam_select_dev(self.dev._h, pl, kind, b, w, v, per_batch, per_beam, ps, pf, int(end_token),
+                                                     1 if normalize else 0, k, po, pp, pp + 8 * b * k))
         return out, beams, tokens
 
     def reorderStates(self, states, parents, lengths=None, time_axis=None, out=None):
@@ -541,33 +549,41 @@ class CUDAAccelerationEngine:
         b, w = parents.shape
         if b == 0 or w == 0:
             raise EmptyInput("no states")
-        if lengths is not None and (not _is_dev(lengths) or lengths.dtype != torch.int64 or tuple(lengths.shape) != (b,)):
+        if lengths is not None and (not _is_dev(lengths) or lengths.dtype != torch.int64 or lengths.shape != (b,)):
             raise InvalidInput("lengths must be a CUDA tensor of int64, [batch]")
         axes = list(time_axis) if isinstance(time_axis, (list, tuple)) else [time_axis] * len(states)
         results = states if out is None else list(out)
         if len(axes) != len(states) or len(results) != len(states):
             raise DimensionMismatch("one time axis and one result per state")
-        moves = (_lib.State * len(states))()
-        for m, t, o, axis in zip(moves, states, results, axes):
+        rows = b * w
+        moves = C.create_string_buffer(_lib.STATE.size * len(states))
+        for i, (t, o, axis) in enumerate(zip(states, results, axes)):
             if not _is_dev(t) or not _is_dev(o):
                 raise InvalidInput("reorderStates takes CUDA tensors")
-            if t.dim() == 0 or t.shape[0] != b * w:
-                raise DimensionMismatch(f"a state must have {b * w} rows, got {tuple(t.shape)}")
-            if o.shape != t.shape or o.dtype != t.dtype:
+            shape = t.shape
+            if len(shape) == 0 or shape[0] != rows:
+                raise DimensionMismatch(f"a state must have {rows} rows, got {tuple(shape)}")
+            if o is not t and (o.shape != shape or o.dtype != t.dtype):
                 raise DimensionMismatch("a result must have its state's shape and type")
             if t.numel() == 0:
                 raise EmptyInput("a state is empty")
-            if axis is not None and not 1 <= axis < t.dim():
-                raise InvalidInput(f"time axis {axis} of a state with {t.dim()} dimensions")
-            outer, inner, steps, per_step, src_outer, dst_outer = _row_parts(t, o, axis if lengths is not None else None)
+            if axis is not None and not 1 <= axis < len(shape):
+                raise InvalidInput(f"time axis {axis} of a state with {len(shape)} dimensions")
+            timed = axis is not None and lengths is not None
             e = t.element_size()
-            m.src, m.dst = t.data_ptr(), o.data_ptr()
-            row = inner * outer
-            m.src_row_stride = (t.stride(0) if b * w > 1 else row) * e
-            m.dst_row_stride = (o.stride(0) if b * w > 1 else row) * e
-            m.src_outer_stride, m.dst_outer_stride = src_outer * e, dst_outer * e
-            m.outer, m.steps, m.step_bytes = outer, steps, per_step * e
-            m.timed = 1 if (axis is not None and lengths is not None) else 0
+            if t.is_contiguous() and (o is t or o.is_contiguous()):
+                src_row = dst_row = t.numel() // rows
+                per_step = src_row
+                for n in shape[1:axis + 1] if timed else ():
+                    per_step //= n
+                steps = shape[axis] if timed else 1
+                src_outer = dst_outer = steps * per_step
+                outer = src_row // src_outer
+            else:
+                outer, inner, steps, per_step, src_outer, dst_outer = _row_parts(t, o, axis if timed else None)
+                src_row, dst_row = (x.stride(0) if rows > 1 else inner * outer for x in (t, o))
+            _lib.STATE.pack_into(moves, i * _lib.STATE.size, t.data_ptr(), o.data_ptr(), src_row * e, dst_row * e, src_outer * e, dst_outer * e,
+                                 outer, steps, per_step * e, 1 if timed else 0, 0)
         parents = parents.contiguous()
         lengths = None if lengths is None else lengths.contiguous()
         pp, pl, *_ = _device_pointers(self.dev, parents, lengths, *states, *(results if out is not None else ()))

@@ -62,55 +62,55 @@ class Int4Quantizer:
                                                _ptr(middles)))
         return codes, scales, middles
 
-    def _descriptor(self, codes, scales, middles, dim, pointers, code_stride, scale_stride):
-        r = _lib.Q4Rows()
-        r.codes, r.scales, r.middles = pointers
-        r.code_stride, r.scale_stride = code_stride, scale_stride
-        r.n, r.dim, r.group = codes.shape[0], dim, self.groupSize
-        return r
+    def _descriptor(self, n, dim, pointers, code_stride, scale_stride):
+        return _lib.Q4Rows(*pointers, code_stride, scale_stride, n, dim, self.groupSize)
 
     def _check(self, codes, scales, middles, dim):
-        if len(codes) == 0:
-            raise EmptyInput("no rows")
         if dim <= 0:
             raise DimensionMismatch("dimension must be positive")
         if self.symmetric != (middles is None):
             raise InvalidInput("a symmetric quantiser has no middles, the other one has")
-        if len(codes.shape) != 2 or codes.shape[1] != (dim + 1) // 2:
-            raise DimensionMismatch(f"expected {(dim + 1) // 2} bytes of codes per row for {dim} columns, got {tuple(codes.shape)}")
-        want = (codes.shape[0], self._groups(dim))
+        shape = codes.shape
+        if len(shape) != 2 or shape[1] != (dim + 1) // 2:
+            raise DimensionMismatch(f"expected {(dim + 1) // 2} bytes of codes per row for {dim} columns, got {tuple(shape)}")
+        if shape[0] == 0:
+            raise EmptyInput("no rows")
+        want = (shape[0], self._groups(dim))
         for name, t in (("scales", scales), ("middles", middles)):
-            if t is not None and tuple(t.shape) != want:
+            if t is not None and t.shape != want:
                 raise DimensionMismatch(f"expected {name} of shape {want}, got {tuple(t.shape)}")
 
     def _device_rows(self, codes, scales, middles, dim):
-        """-> (descriptor's arguments, tensors to keep) for codes and scales in device memory"""
+        """Codes and scales in device memory, checked, with contiguous rows and the strides of the two -> (codes, scales, middles, strides)"""
         self._check(codes, scales, middles, dim)
         for name, t, want in (("codes", codes, torch.uint8), ("scales", scales, torch.float16), ("middles", middles, torch.float16)):
             if t is not None and (not _is_dev(t) or t.dtype != want):
                 raise InvalidInput(f"{name} must be a CUDA tensor of {want}")
         codes, scales = _rows_2d(codes, "codes"), _rows_2d(scales, "scales")
+        per_scales = _row_stride(scales)
         if middles is not None:
             middles = _rows_2d(middles, "middles")
-            if _row_stride(middles) != _row_stride(scales):
+            if _row_stride(middles) != per_scales:
                 scales, middles = scales.contiguous(), middles.contiguous()
-        return codes, scales, middles
+                per_scales = _row_stride(scales)
+        return codes, scales, middles, (_row_stride(codes), per_scales)
 
     def dequantizeBatch(self, codes, scales, middles, dimensions: int):
         """The fp32 values ``[n][dimensions]`` that the codes stand for."""
         dim = int(dimensions)
         if _is_dev(codes):
-            codes, scales, middles = self._device_rows(codes, scales, middles, dim)
+            codes, scales, middles, strides = self._device_rows(codes, scales, middles, dim)
             out = torch.empty((codes.shape[0], dim), dtype=torch.float32, device=codes.device)
             *p, po = _device_pointers(self.dev, codes, scales, middles, out)
-            r = self._descriptor(codes, scales, middles, dim, p, _row_stride(codes), _row_stride(scales))
+            r = self._descriptor(codes.shape[0], dim, p, *strides)
             self.dev.check(self._lib.vsk_q4_decode_dev(self.dev._h, C.byref(r), po))
             return out
         codes, scales = _host(codes, np.uint8), _host(scales, np.float16)
         middles = None if middles is None else _host(middles, np.float16)
         self._check(codes, scales, middles, dim)
         out = np.empty((codes.shape[0], dim), np.float32)
-        r = self._descriptor(codes, scales, middles, dim, [_ptr(codes), _ptr(scales), _ptr(middles)], codes.shape[1], scales.shape[1])
+        p = [None if a is None else a.ctypes.data for a in (codes, scales, middles)]
+        r = self._descriptor(codes.shape[0], dim, p, codes.shape[1], scales.shape[1])
         self.dev.check(self._lib.vsk_q4_decode(self.dev._h, C.byref(r), _ptr(out)))
         return out
 
@@ -123,14 +123,15 @@ class Int4Quantizer:
             raise InvalidInput("product takes CUDA tensors")
         if x.dim() != 2:
             raise DimensionMismatch("x must be a matrix of one vector per row")
-        if x.shape[0] == 0:
+        nq, dim = x.shape
+        if nq == 0:
             raise EmptyInput("no vectors")
-        dim = int(x.shape[1])
-        codes, scales, middles = self._device_rows(codes, scales, middles, dim)
+        codes, scales, middles, strides = self._device_rows(codes, scales, middles, dim)
         x = _rows_2d(x, "x")
-        kind, out_kind = _dtype_id(x.dtype), _dtype_id(out_dtype or x.dtype)
-        y = torch.empty((x.shape[0], codes.shape[0]), dtype=out_dtype or x.dtype, device=x.device)
+        out_dtype = out_dtype or x.dtype
+        kind, out_kind, n = _dtype_id(x.dtype), _dtype_id(out_dtype), codes.shape[0]
+        y = torch.empty((nq, n), dtype=out_dtype, device=x.device)
         *p, px, py = _device_pointers(self.dev, codes, scales, middles, x, y)
-        r = self._descriptor(codes, scales, middles, dim, p, _row_stride(codes), _row_stride(scales))
-        self.dev.check(self._lib.vsk_q4_product_dev(self.dev._h, C.byref(r), px, kind, x.shape[0], _row_stride(x), py, out_kind, y.shape[1]))
+        r = self._descriptor(n, dim, p, *strides)
+        self.dev.check(self._lib.vsk_q4_product_dev(self.dev._h, C.byref(r), px, kind, nq, _row_stride(x), py, out_kind, n))
         return y
