@@ -34,7 +34,7 @@ struct BeamArgs {
   int64_t end_token;
   float2* stats;                  // [batch * beams][pieces]: maximum, sum of exp(x - maximum)
   float* parts;                   // [batch * beams][pieces][parts of one]: maxima of what one load of a warp brings, or null
-  int pieces;
+  int pieces, per_warp;
   float* out_scores;
   int64_t* out_beams;
   int64_t* out_tokens;
@@ -58,59 +58,82 @@ __device__ __forceinline__ float reference_of(float top) { return top == -CUDART
 
 __device__ __forceinline__ float warp_max(float x) { return ordered_to_float(__reduce_max_sync(0xffffffffu, float_to_ordered(x))); }
 
-// ---- one piece per warp -----------------------------------------------------------------------------------------------------
-// 32 x 8 x 131 072 bf16 logits (67 MB): bound by the instructions of a logit (convert, maximum, subtract, multiply, power, add).
+// ---- pieces -------------------------------------------------------------------------------------------------------------------
+template <typename T> __device__ __forceinline__ T lowest();
+template <> __device__ __forceinline__ float lowest<float>() { return -CUDART_INF_F; }
+template <> __device__ __forceinline__ __half lowest<__half>() { return __ushort_as_half(0xfc00); }
+template <> __device__ __forceinline__ __nv_bfloat16 lowest<__nv_bfloat16>() { return __ushort_as_bfloat16(0xff80); }
+
+// A warp takes a.per_warp pieces of a row one after the other, the next one's loads under way.  32 x 8 x 131 072 bf16 logits (67 MB): bound by
+// the instructions of a logit (convert, maximum, convert, subtract, multiply, power, add).
 template <typename T>
 __global__ void __launch_bounds__(256) beam_pieces_kernel(const BeamArgs a) {
   constexpr int kVec = 16 / sizeof(T), kLoads = kPiece / (32 * kVec);
   let_the_next_launch_begin();
   const int lane = threadIdx.x & 31;
-  const int piece = blockIdx.x * 8 + (threadIdx.x >> 5);
+  int piece = (blockIdx.x * 8 + (threadIdx.x >> 5)) * a.per_warp;
   if (piece >= a.pieces) return;
-  const int64_t b = a.first_batch + blockIdx.z, row = b * a.beams + blockIdx.y, item = row * a.pieces + piece;
+  const int end = min(piece + a.per_warp, a.pieces);
+  const int64_t b = a.first_batch + blockIdx.z, row = b * a.beams + blockIdx.y;
   if (!isfinite(__ldg(a.scores + row)) || (a.finished && __ldg(a.finished + row))) return;   // not looked at again
   const T* base = reinterpret_cast<const T*>(a.logits) + b * a.batch_stride + blockIdx.y * a.beam_stride;
   // pieces begin at 16-byte boundaries of the address, so the first one of a row may begin before it
-  const int64_t first = (int64_t)piece * kPiece - (int64_t)((reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T));
-  float x[kLoads * kVec];
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int64_t at = first + (i * 32 + lane) * kVec;
-    if (at >= 0 && at + kVec <= a.vocab) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(base + at));
-      const T* h = reinterpret_cast<const T*>(&v);
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) x[i * kVec + j] = as_float<T>(h[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) x[i * kVec + j] = at + j >= 0 && at + j < a.vocab ? as_float<T>(*VSK_CHK(base + at + j)) : -CUDART_INF_F;
-    }
-  }
-  float own[kLoads], top = -CUDART_INF_F;
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    own[i] = -CUDART_INF_F;
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) own[i] = fmaxf(own[i], x[i * kVec + j]);   // (a NaN is passed over)
-    top = fmaxf(top, own[i]);
-  }
-  top = warp_max(top);
-  if (a.parts) {
+  const int before = (int)((reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T));
+  auto load = [&](int p, uint4 (&raw)[kLoads]) {
+    const int64_t first = (int64_t)p * kPiece - before + lane * kVec;
+    const T* src = base + first;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const float m = warp_max(own[i]);
-      if (lane == i) *VSK_CHK_W(a.parts + item * kLoads + i) = m;
+      const int64_t at = first + i * 32 * kVec;
+      if (at >= 0 && at + kVec <= a.vocab) {
+        raw[i] = __ldg(reinterpret_cast<const uint4*>(src + i * 32 * kVec));
+      } else {
+        __align__(16) T h[kVec];
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) h[j] = at + j >= 0 && at + j < a.vocab ? *VSK_CHK(base + at + j) : lowest<T>();
+        raw[i] = *reinterpret_cast<const uint4*>(h);
+      }
     }
-  }
-  float sum = 0.f;
-  if (a.normalize) {
-    const float from = reference_of(top);   // (+inf stays: its row's sum becomes NaN, and so does a NaN's)
+  };
+  uint4 next[kLoads];
+  load(piece, next);
+  for (; piece < end; ++piece) {
+    uint4 raw[kLoads];
 #pragma unroll
-    for (int i = 0; i < kLoads * kVec; ++i) sum += exp_of(x[i], from);
+    for (int i = 0; i < kLoads; ++i) raw[i] = next[i];
+    if (piece + 1 < end) load(piece + 1, next);
+    float own[kLoads], top = -CUDART_INF_F;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int i = 0; i < kLoads; ++i) {
+      const T* h = reinterpret_cast<const T*>(&raw[i]);
+      own[i] = -CUDART_INF_F;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) own[i] = fmaxf(own[i], as_float<T>(h[j]));   // (a NaN is passed over)
+      top = fmaxf(top, own[i]);
+    }
+    top = warp_max(top);
+    const int64_t item = row * a.pieces + piece;
+    if (a.parts) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const float m = warp_max(own[i]);
+        if (lane == i) *VSK_CHK_W(a.parts + item * kLoads + i) = m;
+      }
+    }
+    float sum = 0.f;
+    if (a.normalize) {
+      const float from = reference_of(top);   // (+inf stays: its row's sum becomes NaN, and so does a NaN's)
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const T* h = reinterpret_cast<const T*>(&raw[i]);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) sum += exp_of(as_float<T>(h[j]), from);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    if (lane == 0) *VSK_CHK_W(a.stats + item) = make_float2(top, sum);
   }
-  if (lane == 0) *VSK_CHK_W(a.stats + item) = make_float2(top, sum);
 }
 
 // ---- selection --------------------------------------------------------------------------------------------------------------
@@ -457,9 +480,11 @@ int32_t select(Ctx* ctx, BeamArgs a) {
   VSK_TRY(scratch(ctx, SLOT_BEAM, (size_t)items * (sizeof(float2) + (parts ? kParts * sizeof(float) : 0)), &p));
   a.stats = (float2*)p;
   a.parts = parts ? (float*)(a.stats + items) : nullptr;
+  // as many pieces per warp as leave two rounds of warps
+  a.per_warp = (int)std::max<int64_t>(1, std::min<int64_t>(8, items / ((int64_t)ctx->prop.multiProcessorCount * 64)));
   for (int64_t f = 0; f < a.batch; f += 65535) {
     a.first_batch = f;
-    beam_pieces_kernel<T><<<dim3((unsigned)ceil_div(a.pieces, 8), (unsigned)a.beams, (unsigned)std::min<int64_t>(65535, a.batch - f)), 256, 0,
+    beam_pieces_kernel<T><<<dim3((unsigned)ceil_div(a.pieces, 8 * a.per_warp), (unsigned)a.beams, (unsigned)std::min<int64_t>(65535, a.batch - f)), 256, 0,
                            ctx->stream>>>(a);
     ctx->stats.kernel_launches++;
     VSK_CUDA(ctx, cudaGetLastError());
