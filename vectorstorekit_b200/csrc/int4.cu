@@ -24,122 +24,177 @@ template <> __device__ __forceinline__ float to_float<__half>(__half v) { return
 template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
 // ---- encoding -----------------------------------------------------------------------------------------------------------
-// One warp per 128 columns of a row, four columns per lane: a group of G columns is G / 4 lanes, its extremes a few shuffles.
+// Eight columns per lane: a group of G columns is G / 8 lanes, its extremes a few shuffles.  `lanes` neighbouring lanes share a row (short
+// rows leave several to a warp) and walk along it, the next columns' load under way.  100 000 x 768 fp32, groups of 32, min / max:
+// bound by the instructions of a value, of which the 64-bit ones are kept to what the definition needs.
 
-// The whole number nearest to away / step in 64 bits, ties to even.  The fp32 quotient is off by less than 1e-5 where the code is not
-// clipped anyway (|quotient| < 9, three roundings of 2^-24 each): only quotients that near to a half are divided in 64 bits.
-__device__ __forceinline__ int nearest_code(float x, float mid, float inv, float step) {
-  const float u = (x - mid) * inv;
-  float r = rintf(u);
-  if (fabsf(u) < 9.0f && fabsf(u - r) > 0.5f - 1e-5f) r = (float)rint(((double)x - (double)mid) / (double)step);
-  return (int)fminf(fmaxf(r, -8.0f), 7.0f) + 8;
+// (float)(d / 15) with the quotient in 64 bits.  The product with the rounded reciprocal is off by less than 2 of its last bits: it
+// rounds to the same fp32 number unless it lies that near to the middle between two.
+__device__ __forceinline__ float fifteenth(double d) {
+  const double q = d * (1.0 / 15.0);
+  const int rest = (int)(__double2loint(q) & 0x1fffffff) - 0x10000000;   // the 29 bits that fp32 drops (normal numbers)
+  if (abs(rest) < 8 || !(q > 1.2e-38)) return (float)(d / 15.0);
+  return (float)q;
 }
 
-template <typename T>
+// Eight codes, the first in the lowest four bits: the whole numbers nearest to (x - mid) / step in 64 bits, ties to even, within -8 .. 7.  The
+// fp32 quotient is off by less than 1e-5 there (a few roundings of 2^-24 each): only where one lies that near to a half are they divided
+// in 64 bits.  Rounding and conversion are an addition of 1.5 2^23: the unit that has instructions for them takes a quarter of the rate.
+__device__ __forceinline__ unsigned nearest_codes(const float (&x)[8], float mid, float inv, float step) {
+  unsigned t[8];
+  float far = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float u = fminf(fmaxf((x[j] - mid) * inv, -8.f), 7.f), r = u + 12582912.f;
+    far = fmaxf(far, fabsf(u - (r - 12582912.f)));
+    t[j] = __float_as_uint(r);
+  }
+  if (far > 0.5f - 1e-5f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = (unsigned)(int)fmin(fmax(rint(((double)x[j] - (double)mid) / (double)step), -8.0), 7.0);
+  }
+  unsigned c = 0x88888888u;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c ^= (t[j] & 15u) << (4 * j);
+  return c;
+}
+
+template <typename T, bool SYMMETRIC>
 __global__ void __launch_bounds__(256) q4_encode_kernel(const T* __restrict__ rows, int64_t n, int dim, int64_t row_stride, int group,
-                                                        int groups, int symmetric, int wide, uint8_t* __restrict__ codes,
+                                                        int groups, int lanes, int columns, int wide, uint8_t* __restrict__ codes,
                                                         int64_t code_stride, __half* __restrict__ scales,
                                                         __half* __restrict__ middles) {
-  const int lane = threadIdx.x & 31;
-  const int pieces = (dim + 127) / 128;
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (item >= n * pieces) return;   // (whole warps)
-  const int64_t row = item / pieces;
-  const int col = (int)(item - row * pieces) * 128 + lane * 4;
-  const T* src = rows + row * row_stride + col;
-  float v[4];
-  const int have = max(0, min(4, dim - col));
-  if (wide && have == 4) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 f = __ldg(reinterpret_cast<const float4*>(src));
-      v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+  const int lane = threadIdx.x & (lanes - 1), per_block = 256 / lanes;
+  const int64_t row = (int64_t)blockIdx.x * per_block + threadIdx.x / lanes;
+  const bool inside = row < n;   // (whole warps walk together)
+  const T* const src = rows + (inside ? row : 0) * row_stride;
+  uint8_t* const dst = codes + (inside ? row : 0) * code_stride;
+  const bool words = (code_stride & 3) == 0 && (reinterpret_cast<uintptr_t>(codes) & 3) == 0;
+  const int first = blockIdx.y * columns, end = min(dim, first + columns), stride = 8 * lanes;
+  const int group_shift = group == 32 ? 5 : group == 64 ? 6 : 7;
+
+  auto load = [&](int col, float (&v)[8]) {
+    const int have = inside ? min(8, end - col) : 0;
+    if (wide && have == 8) {
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+          const float4 f = __ldg(reinterpret_cast<const float4*>(src + col + j));
+          v[j] = f.x; v[j + 1] = f.y; v[j + 2] = f.z; v[j + 3] = f.w;
+        }
+      } else {
+        const uint4 f = __ldg(reinterpret_cast<const uint4*>(src + col));
+        const T* h = reinterpret_cast<const T*>(&f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = to_float<T>(h[j]);
+      }
     } else {
-      const uint2 f = __ldg(reinterpret_cast<const uint2*>(src));
-      const T* h = reinterpret_cast<const T*>(&f);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = to_float<T>(h[j]);
+      for (int j = 0; j < 8; ++j) v[j] = j < have ? to_float<T>(*VSK_CHK(src + col + j)) : j == 0 ? 0.f : v[0];   // (no other extremes)
     }
-  } else {
+  };
+  float next[8];
+  load(first + lane * 8, next);
+  for (int base = first; base < end; base += stride) {
+    const int col = base + lane * 8;
+    float v[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = j < have ? to_float<T>(*VSK_CHK(src + j)) : 0.f;
-  }
-  float hi = -CUDART_INF_F, lo = CUDART_INF_F;
+    for (int j = 0; j < 8; ++j) v[j] = next[j];
+    if (base + stride < end) load(col + stride, next);
+    const int have = inside ? min(8, end - col) : 0;
+    float hi = v[0], lo = v[0];
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (j < have) {
+    for (int j = 1; j < 8; ++j) {
       hi = fmaxf(hi, v[j]);
       lo = fminf(lo, v[j]);
     }
-  for (int o = group / 8; o > 0; o >>= 1) {
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-  }
-  if (have == 0) return;   // (no shuffles behind this)
-  // two roundings, to fp32 and to fp16, as a host computes them
-  float step, mid = 0.f;
-  if (symmetric) {
-    step = (float)((double)fmaxf(hi, -lo) / 7.0);
-  } else {
-    step = (float)(((double)hi - (double)lo) / 15.0);
-  }
-  const __half hs = __float2half_rn(fminf(step, 65504.f));
-  step = __half2float(hs);
-  const int64_t slot = row * groups + col / group;
-  const bool first = (col % group) == 0;
-  if (!symmetric) {
-    const float m = (float)((double)lo + 8.0 * (double)step);
-    const __half hm = __float2half_rn(fminf(fmaxf(m, -65504.f), 65504.f));
-    mid = __half2float(hm);
-    if (first) *VSK_CHK_W(middles + slot) = hm;
-  }
-  if (first) *VSK_CHK_W(scales + slot) = hs;
-  const float inv = 1.0f / step;
-  int c[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) c[j] = (j < have && step > 0.f) ? nearest_code(v[j], mid, inv, step) : 8;
-  uint8_t* dst = codes + row * code_stride + (col >> 1);
-  const uint8_t b0 = (uint8_t)(c[0] | (c[1] << 4)), b1 = (uint8_t)(c[2] | (c[3] << 4));
-  if (have > 2 && (code_stride & 1) == 0 && (reinterpret_cast<uintptr_t>(codes) & 1) == 0) {
-    *VSK_CHK_W(reinterpret_cast<uint16_t*>(dst)) = (uint16_t)(b0 | (b1 << 8));
-  } else {
-    *VSK_CHK_W(dst) = b0;
-    if (have > 2) *VSK_CHK_W(dst + 1) = b1;
+    if (have <= 0) {
+      hi = -CUDART_INF_F;
+      lo = CUDART_INF_F;
+    }
+    if (SYMMETRIC) hi = fmaxf(hi, -lo);
+    for (int o = group / 16; o > 0; o >>= 1) {
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      if (!SYMMETRIC) lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    }
+    if (have <= 0) continue;
+    // Two roundings, to fp32 and to fp16, as a host computes them from the quotient in 64 bits.  (A seventh of an fp32 number is never
+    // nearer than 2^-28 of it to the middle between two: one division in fp32 rounds alike.)
+    float step, mid = 0.f;
+    if (SYMMETRIC) step = __fdiv_rn(hi, 7.0f);
+    else step = fifteenth((double)hi - (double)lo);
+    const __half hs = __float2half_rn(fminf(step, 65504.f));
+    step = __half2float(hs);
+    const int64_t slot = row * groups + (col >> group_shift);
+    const bool leads = (col & (group - 1)) == 0;
+    if (!SYMMETRIC) {
+      const float m = (float)((double)lo + 8.0 * (double)step);
+      const __half hm = __float2half_rn(fminf(fmaxf(m, -65504.f), 65504.f));
+      mid = __half2float(hm);
+      if (leads) *VSK_CHK_W(middles + slot) = hm;
+    }
+    if (leads) *VSK_CHK_W(scales + slot) = hs;
+    const float inv = step > 0.f ? __fdividef(1.0f, step) : 0.f;   // (of an fp16 number: in range)
+    unsigned c = nearest_codes(v, mid, inv, step);
+    uint8_t* const at = dst + (col >> 1);
+    if (have == 8 && words) {
+      *VSK_CHK_W(reinterpret_cast<uint32_t*>(at)) = c;
+    } else {
+      if (have & 1) c = (c & ~(15u << (4 * have))) | (8u << (4 * have));   // the half behind an odd last column
+      for (int j = 0; j < (have + 1) / 2; ++j) *VSK_CHK_W(at + j) = (uint8_t)(c >> (8 * j));
+    }
   }
 }
 
-// ---- decoding: one thread per eight columns --------------------------------------------------------------------------------
+// ---- decoding: eight columns per thread, `lanes` threads along a row -------------------------------------------------------------
+constexpr int kDecodeSteps = 4;
 __global__ void __launch_bounds__(256) q4_decode_kernel(const uint8_t* __restrict__ codes, int64_t code_stride,
                                                         const __half* __restrict__ scales, const __half* __restrict__ middles,
-                                                        int64_t scale_stride, int64_t n, int dim, int group,
+                                                        int64_t scale_stride, int64_t n, int dim, int group_shift, int lanes, int columns,
                                                         float* __restrict__ out) {
-  const int pieces = (dim + 7) / 8;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n * pieces) return;
-  const int64_t row = i / pieces;
-  const int col = (int)(i - row * pieces) * 8;
-  const uint8_t* src = codes + row * code_stride + (col >> 1);
-  const int have = min(8, dim - col);
-  uint32_t w = 0;
-  if (have == 8 && (reinterpret_cast<uintptr_t>(src) & 3) == 0) {
-    w = __ldg(reinterpret_cast<const uint32_t*>(src));
-  } else {
-    for (int j = 0; j < (have + 1) / 2; ++j) w |= (uint32_t)*VSK_CHK(src + j) << (8 * j);
-  }
-  const int64_t slot = row * scale_stride + col / group;
-  const float s = __half2float(*VSK_CHK(scales + slot));
-  const float m = middles ? __half2float(*VSK_CHK(middles + slot)) : 0.f;
-  float v[8];
+  const int64_t row = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+  if (row >= n) return;
+  const uint8_t* const line = codes + row * code_stride;
+  const __half* const s_line = scales + row * scale_stride;
+  const __half* const m_line = middles + row * scale_stride;
+  float* const to = out + row * dim;
+  const int end = min(dim, ((int)blockIdx.y + 1) * columns), first = blockIdx.y * columns + (threadIdx.x & (lanes - 1)) * 8;
+  // everything that a thread needs is asked for before anything is stored (`columns` are at most as many strides)
+  uint32_t w[kDecodeSteps];
+  __half s[kDecodeSteps], m[kDecodeSteps];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    v[j] = s * (float)((int)((w >> (4 * j)) & 15) - 8);   // exact: 11 + 4 bits
-    if (middles) v[j] = __fadd_rn(v[j], m);
+  for (int i = 0; i < kDecodeSteps; ++i) {
+    const int col = first + i * lanes * 8, have = min(8, end - col);
+    w[i] = 0;
+    s[i] = m[i] = __half(0.f);
+    if (have <= 0) continue;
+    const uint8_t* src = line + (col >> 1);
+    if (have == 8 && (reinterpret_cast<uintptr_t>(src) & 3) == 0) {
+      w[i] = __ldg(reinterpret_cast<const uint32_t*>(src));
+    } else {
+      for (int j = 0; j < (have + 1) / 2; ++j) w[i] |= (uint32_t)*VSK_CHK(src + j) << (8 * j);
+    }
+    s[i] = *VSK_CHK(s_line + (col >> group_shift));
+    if (middles) m[i] = *VSK_CHK(m_line + (col >> group_shift));
   }
-  float* dst = out + row * dim + col;
-  if (have == 8 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-    reinterpret_cast<float4*>(VSK_CHK_W(dst))[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(VSK_CHK_W(dst + 4))[0] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-    for (int j = 0; j < have; ++j) *VSK_CHK_W(dst + j) = v[j];
+#pragma unroll
+  for (int i = 0; i < kDecodeSteps; ++i) {
+    const int col = first + i * lanes * 8, have = min(8, end - col);
+    if (have <= 0) continue;
+    const float scale = __half2float(s[i]), middle = __half2float(m[i]);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = scale * (float)((int)((w[i] >> (4 * j)) & 15) - 8);   // exact: 11 + 4 bits
+      if (middles) v[j] = __fadd_rn(v[j], middle);
+    }
+    float* dst = to + col;
+    if (have == 8 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+      *VSK_CHK_W(reinterpret_cast<float4*>(dst)) = make_float4(v[0], v[1], v[2], v[3]);
+      *VSK_CHK_W(reinterpret_cast<float4*>(dst + 4)) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      for (int j = 0; j < have; ++j) *VSK_CHK_W(dst + j) = v[j];
+    }
   }
 }
 
@@ -175,14 +230,18 @@ int dtype_size(int32_t t) { return t == VSK_DTYPE_F32 ? 4 : (t == VSK_DTYPE_F16 
 int32_t encode(Ctx* ctx, const void* rows, int32_t dtype, int64_t n, int32_t dim, int64_t row_stride, int32_t group, int32_t symmetric,
                uint8_t* codes, int64_t code_stride, void* scales, void* middles) {
   const int es = dtype_size(dtype);
-  const int64_t items = n * ceil_div(dim, 128), blocks = ceil_div(items, 8);
-  if (blocks > 0x7fffffffLL) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "too many rows in one call");
   const int groups = (int)ceil_div(dim, group);
-  const int wide = ((reinterpret_cast<uintptr_t>(rows) | (uintptr_t)(row_stride * es)) & (uintptr_t)(4 * es - 1)) == 0;
+  const int wide = ((reinterpret_cast<uintptr_t>(rows) | (uintptr_t)(row_stride * es)) & 15) == 0;
+  int lanes = group / 8;
+  while (lanes < 32 && lanes * 8 < dim) lanes *= 2;
+  const int columns = 1024;   // of a thread's walk: a multiple of every stride and group
+  const int64_t blocks = ceil_div(n, 256 / lanes), along = ceil_div(dim, columns);
+  if (blocks > 0x7fffffffLL) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "too many rows in one call");
   auto go = [&](auto* x) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
-    q4_encode_kernel<T><<<(unsigned)blocks, 256, 0, ctx->stream>>>(x, n, dim, row_stride, group, groups, symmetric, wide, codes,
-                                                                   code_stride, (__half*)scales, (__half*)middles);
+    const dim3 grid((unsigned)blocks, (unsigned)along);
+    if (symmetric) q4_encode_kernel<T, true><<<grid, 256, 0, ctx->stream>>>(x, n, dim, row_stride, group, groups, lanes, columns, wide, codes, code_stride, (__half*)scales, nullptr);
+    else q4_encode_kernel<T, false><<<grid, 256, 0, ctx->stream>>>(x, n, dim, row_stride, group, groups, lanes, columns, wide, codes, code_stride, (__half*)scales, (__half*)middles);
   };
   if (dtype == VSK_DTYPE_F32) go((const float*)rows);
   else if (dtype == VSK_DTYPE_F16) go((const __half*)rows);
@@ -193,10 +252,14 @@ int32_t encode(Ctx* ctx, const void* rows, int32_t dtype, int64_t n, int32_t dim
 }
 
 int32_t decode(Ctx* ctx, const vsk_q4_rows* r, float* out) {
-  const int64_t blocks = ceil_div(r->n * ceil_div(r->dim, 8), 256);
+  int lanes = 1;
+  while (lanes < 32 && lanes * 8 < r->dim) lanes *= 2;
+  const int columns = kDecodeSteps * lanes * 8;
+  const int64_t blocks = ceil_div(r->n, 256 / lanes);
   if (blocks > 0x7fffffffLL) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "too many rows in one call");
-  q4_decode_kernel<<<(unsigned)blocks, 256, 0, ctx->stream>>>(r->codes, r->code_stride, (const __half*)r->scales,
-                                                              (const __half*)r->middles, r->scale_stride, r->n, r->dim, r->group, out);
+  q4_decode_kernel<<<dim3((unsigned)blocks, (unsigned)ceil_div(r->dim, columns)), 256, 0, ctx->stream>>>(
+      r->codes, r->code_stride, (const __half*)r->scales, (const __half*)r->middles, r->scale_stride, r->n, r->dim,
+      r->group == 32 ? 5 : r->group == 64 ? 6 : 7, lanes, columns, out);
   ctx->stats.kernel_launches++;
   VSK_CUDA(ctx, cudaGetLastError());
   return VSK_OK;
