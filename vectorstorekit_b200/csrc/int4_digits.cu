@@ -468,30 +468,59 @@ __global__ void __launch_bounds__(32 * kWarps, DT == 4 ? 1 : 2) q4_digits_kernel
   }
 }
 
-// One block per vector: its largest element, then digits in the order of the fragments, and its sums over the groups.
+// One block per vector: its largest element, then digits in the order of the fragments, and its sums over the groups.  Eight columns per
+// thread; of vectors of up to 8 192 nothing is read twice.
+constexpr int kToDigits = 512, kKept = 2;
 template <typename X>
-__global__ void __launch_bounds__(256) q4_to_digits_kernel(const X* __restrict__ x, int64_t x_stride, int dim, int ksteps, int digits, int per_launch,
-                                                           int tiles, int group, uint2* __restrict__ frags, float* __restrict__ sums,
-                                                           int sum_stride, VectorInfo* __restrict__ info) {
-  __shared__ float warp_top[8];
+__global__ void __launch_bounds__(kToDigits) q4_to_digits_kernel(const X* __restrict__ x, int64_t x_stride, int wide, int dim, int ksteps, int digits,
+                                                                 int per_launch, int tiles, int group, uint2* __restrict__ frags,
+                                                                 float* __restrict__ sums, int sum_stride, VectorInfo* __restrict__ info) {
+  __shared__ float warp_top[kToDigits / 32];
   __shared__ int wrong;
   let_the_next_launch_begin();
   const int64_t q = blockIdx.x;
   const X* src = x + q * x_stride;
-  auto value = [&](int i) {
-    const X e = *VSK_CHK(src + i);
+  auto to_f32 = [](X e) {
     if constexpr (std::is_same<X, float>::value) return e;
     else if constexpr (std::is_same<X, __half>::value) return __half2float(e);
     else return __bfloat162float(e);
+  };
+  auto load = [&](int col, float (&v)[8]) {
+    if (wide && col + 8 <= dim) {
+      constexpr int kVec = 16 / sizeof(X);
+#pragma unroll
+      for (int j = 0; j < 8; j += kVec) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(src + col + j));
+        const X* h = reinterpret_cast<const X*>(&u);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) v[j + e] = to_f32(h[e]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = col + j < dim ? to_f32(*VSK_CHK(src + col + j)) : 0.f;
+    }
   };
   if (threadIdx.x == 0) wrong = 0;
   __syncthreads();
   float top = 0.f;
   bool bad = false;
-  for (int i = threadIdx.x; i < dim; i += 256) {
-    const float v = value(i);
-    bad |= !isfinite(v);
-    top = fmaxf(top, fabsf(v));
+  float kept[kKept][8];
+  auto look = [&](const float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      bad |= !isfinite(v[j]);
+      top = fmaxf(top, fabsf(v[j]));
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) {
+    load((i * kToDigits + (int)threadIdx.x) * 8, kept[i]);
+    look(kept[i]);
+  }
+  for (int col = (kKept * kToDigits + (int)threadIdx.x) * 8; col < dim; col += kToDigits * 8) {
+    float v[8];
+    load(col, v);
+    look(v);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -499,7 +528,7 @@ __global__ void __launch_bounds__(256) q4_to_digits_kernel(const X* __restrict__
   if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 8; ++w) top = fmaxf(top, warp_top[w]);
+  for (int w = 0; w < kToDigits / 32; ++w) top = fmaxf(top, warp_top[w]);
   const bool finite = wrong == 0;
   // the largest power of two that keeps |top| within 127 256^(digits-1) + ... + 127
   const float most = digits == 4 ? 2139062144.f - 128.f : 8355711.f;
@@ -513,16 +542,15 @@ __global__ void __launch_bounds__(256) q4_to_digits_kernel(const X* __restrict__
   const float up0 = ldexpf(1.f, max(-126, min(127, shift))), up1 = ldexpf(1.f, shift - max(-126, min(127, shift)));
   const int64_t chunk = q / per_launch;
   const int first_col = (int)(q % per_launch) * digits;
-  for (int p0 = 0; p0 < ksteps * 16; p0 += 256) {   // (whole warps stay together for the sums)
-    const int p = p0 + (int)threadIdx.x, col = p * 8;   // eight columns
+  auto put = [&](int p, const float (&v)[8]) {   // (whole warps together, for the sums)
+    const int col = p * 8;
     const bool inside = p < ksteps * 16;
     uint32_t even[4] = {}, odd[4] = {};
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float v = finite && col + j < dim ? value(col + j) : 0.f;
-      s += v;
-      int n = __float2int_rn(v * up0 * up1);
+      s += v[j];
+      int n = __float2int_rn(v[j] * up0 * up1);
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
         if (d == digits) break;
@@ -547,6 +575,23 @@ __global__ void __launch_bounds__(256) q4_to_digits_kernel(const X* __restrict__
       for (int o = group / 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       if (inside && col % group == 0) *VSK_CHK_W(sums + q * sum_stride + col / group) = s;
     }
+  };
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) {
+    if (!finite) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) kept[i][j] = 0.f;   // (the product kernel does without)
+    }
+    if (i * kToDigits < ksteps * 16) put(i * kToDigits + (int)threadIdx.x, kept[i]);
+  }
+  for (int p0 = kKept * kToDigits; p0 < ksteps * 16; p0 += kToDigits) {
+    float v[8];
+    load((p0 + (int)threadIdx.x) * 8, v);
+    if (!finite) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    }
+    put(p0 + (int)threadIdx.x, v);
   }
 }
 
@@ -633,7 +678,8 @@ int32_t q4_product_digits(Ctx* ctx, const vsk_q4_rows& rows, const void* x, int3
   a.info = info;
   auto prepare = [&](auto* v) {
     using X = std::remove_const_t<std::remove_pointer_t<decltype(v)>>;
-    q4_to_digits_kernel<X><<<(unsigned)nq, 256, 0, ctx->stream>>>(v, x_stride, a.dim, a.ksteps, a.digits, a.per_launch, tiles, a.group, (uint2*)p, sums,
+    const int wide = ((reinterpret_cast<uintptr_t>(v) | (uintptr_t)(x_stride * sizeof(X))) & 15) == 0;
+    q4_to_digits_kernel<X><<<(unsigned)nq, kToDigits, 0, ctx->stream>>>(v, x_stride, wide, a.dim, a.ksteps, a.digits, a.per_launch, tiles, a.group, (uint2*)p, sums,
                                                                   a.sum_stride, info);
   };
   if (x_dtype == VSK_DTYPE_F32) prepare((const float*)x);
