@@ -550,8 +550,9 @@ int32_t vsk_pq_index_add_dev(vsk_index* index, const uint8_t* codes, int64_t n);
  *   decode      -> out[n][dim] fp32, each value rounded once
  *   product     y[q * y_stride + r] = sum over the columns of value(r, i) x[q * x_stride + i]: the scores of nq vectors
  *               against all rows, as a decoding step takes them from a projection or an output head, or a query from a store
- *               (dotProduct negates them).  Sums in fp32, rounded once to y's type.  fp32 vectors are taken exactly.  Finite vectors
- *               with elements below 2^120.  x and y must not overlap. */
+ *               (dotProduct negates them).  Sums in fp32, rounded once to y's type.  fp32 vectors, and up to four 16-bit ones,
+ *               are taken to 2^-31 of their largest element, others exactly.  Elements below 2^120; an infinity or a NaN stays in
+ *               its vector's products.  x and y must not overlap. */
 typedef enum vsk_dtype { VSK_DTYPE_F32 = 0, VSK_DTYPE_F16 = 1, VSK_DTYPE_BF16 = 2 } vsk_dtype;
 typedef struct vsk_q4_rows {
   const uint8_t* codes;

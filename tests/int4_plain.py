@@ -45,12 +45,14 @@ def product_bound(codes, scales, middles, group, x, y, out):
     """How far a product in fp32 sums may be from the exact y.  A group's sum is a chain of at most `group` additions per part of x,
     the groups one multiply-add each (two with middles), the parts and the shares of eight warps a dozen more; the sums of x over a group
     chain `group` additions too.  Each addition loses at most 2^-23 (a unit that cuts off rather than rounds) of a partial sum, and no partial
-    sum is larger than the sum of the magnitudes.  Then one rounding to the result's type."""
+    sum is larger than the sum of the magnitudes.  A vector may be held in whole numbers of 2^-30 of its largest element (31 bits): half of
+    that per element.  Then one rounding to the result's type."""
     dim = codes.shape[1]
     mag = np.abs(codes - 8.0) * np.repeat(np.abs(scales.astype(np.float64)), group, 1)[:, :dim]
     if middles is not None:
         mag = mag + np.repeat(np.abs(middles.astype(np.float64)), group, 1)[:, :dim]
     steps = 2 * group + 2 * scales.shape[1] + 16
-    sums = np.abs(x.astype(np.float64)) @ mag.T
+    x = np.abs(x.astype(np.float64))
+    sums, grid = x @ mag.T, 2.0 ** -31 * np.max(x, axis=1, keepdims=True) * np.sum(mag, axis=1)
     rel, tiny = HALF[out]
-    return steps * 2.0 ** -23 * sums * (1 + rel) + rel * np.abs(y) + tiny
+    return (steps * 2.0 ** -23 * sums + grid) * (1 + rel) + rel * np.abs(y) + tiny

@@ -197,6 +197,24 @@ def test_products_of_unusual_vectors(dev):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_products_of_vectors_with_one_element_far_above_the_others(dev, kind):
+    """A thousand times the others, as activations of language models have them; rows with and without a weight at that place."""
+    import torch
+    rng = np.random.default_rng(13)
+    codes, scales, middles = _case(rng, 80, 512, 64, True)
+    codes[::2, 77] = 8
+    for nq in (1, 4, 5, 9):
+        x = torch.from_numpy(rng.standard_normal((nq, 512))).to(_t(kind))
+        x[:, 77] = 1000.0
+        got = _run(dev, codes, scales, middles, 64, x, "f32")
+        _compare(got, codes, scales, middles, 64, x, "f32")
+        # the rows without that weight: no worse than an fp32 sum of what they hold
+        small = x.clone()
+        small[:, 77] = 0
+        _compare(got[:, ::2], codes[::2], scales[::2], middles, 64, small, "f32")
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 def test_infinities_and_nan_in_one_vector_stay_in_its_products(dev, kind):
     import torch
     rng = np.random.default_rng(12)

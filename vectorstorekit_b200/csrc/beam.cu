@@ -650,6 +650,7 @@ int32_t vsk_beam_select_dev(vsk_ctx* c, const void* logits, int32_t dtype, int64
   a.out_beams = out_beams;
   a.out_tokens = out_tokens;
   VSK_TRY(dtype == VSK_DTYPE_F32 ? select<float>(ctx, a) : dtype == VSK_DTYPE_F16 ? select<__half>(ctx, a) : select<__nv_bfloat16>(ctx, a));
+  tl_mark(ctx, "beam_select");
   VSK_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
   return VSK_OK;
 }
@@ -717,6 +718,7 @@ int32_t vsk_reorder_states_dev(vsk_ctx* c, const vsk_state* states, int32_t coun
         a.count = 0;
       }
     }
+  tl_mark(ctx, "reorder_states");
   VSK_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
   if (*bad) return fail(ctx, VSK_ERR_INVALID_INPUT, "a parent is outside [-1, %d): its batch entry's states were left as they were", beams);
   return VSK_OK;

@@ -310,6 +310,7 @@ int32_t vsk_q4_encode_dev(vsk_ctx* c, const void* rows, int32_t dtype, int64_t n
   VSK_TRY(check_encode(ctx, rows, dtype, n, dim, row_stride, group, symmetric, codes, code_stride, scales, middles));
   drain_stale_error("vsk_q4_encode_dev");
   VSK_TRY(encode(ctx, rows, dtype, n, dim, row_stride, group, symmetric, codes, code_stride, scales, middles));
+  tl_mark(ctx, "q4_encode");
   VSK_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
   return VSK_OK;
 }
@@ -321,7 +322,8 @@ int32_t vsk_q4_encode(vsk_ctx* c, const float* rows, int64_t n, int32_t dim, int
   VSK_TRY(check_ctx(c, &ctx));
   VSK_TRY(check_encode(ctx, rows, VSK_DTYPE_F32, n, dim, dim, group, symmetric, codes, code_stride, scales, middles));
   drain_stale_error("vsk_q4_encode");
-  const size_t in = (size_t)n * dim * 4, held = (size_t)n * code_stride, per = (size_t)n * ceil_div(dim, group) * 2;
+  const int64_t width = (dim + 1) / 2;
+  const size_t in = (size_t)n * dim * 4, held = (size_t)n * width, per = (size_t)n * ceil_div(dim, group) * 2;
   Staged s(ctx);
   void *dx, *dc, *ds, *dm = nullptr;
   VSK_TRY(s.get(in, &dx));
@@ -329,10 +331,9 @@ int32_t vsk_q4_encode(vsk_ctx* c, const float* rows, int64_t n, int32_t dim, int
   VSK_TRY(s.get(per, &ds));
   if (!symmetric) VSK_TRY(s.get(per, &dm));
   VSK_CUDA(ctx, cudaMemcpyAsync(dx, rows, in, cudaMemcpyHostToDevice, ctx->stream));
-  // (bytes of a code row behind its columns are the caller's: they go back as zeros of this copy)
-  VSK_CUDA(ctx, cudaMemsetAsync(dc, 0, held, ctx->stream));
-  VSK_TRY(encode(ctx, dx, VSK_DTYPE_F32, n, dim, dim, group, symmetric, (uint8_t*)dc, code_stride, ds, dm));
-  VSK_CUDA(ctx, cudaMemcpyAsync(codes, dc, held, cudaMemcpyDeviceToHost, ctx->stream));
+  VSK_TRY(encode(ctx, dx, VSK_DTYPE_F32, n, dim, dim, group, symmetric, (uint8_t*)dc, width, ds, dm));
+  // (bytes of a code row behind its columns are the caller's)
+  VSK_CUDA(ctx, cudaMemcpy2DAsync(codes, (size_t)code_stride, dc, (size_t)width, (size_t)width, (size_t)n, cudaMemcpyDeviceToHost, ctx->stream));
   VSK_CUDA(ctx, cudaMemcpyAsync(scales, ds, per, cudaMemcpyDeviceToHost, ctx->stream));
   if (!symmetric) VSK_CUDA(ctx, cudaMemcpyAsync(middles, dm, per, cudaMemcpyDeviceToHost, ctx->stream));
   VSK_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
@@ -349,6 +350,7 @@ int32_t vsk_q4_decode_dev(vsk_ctx* c, const vsk_q4_rows* rows, float* out) {
   if (!out) return fail(ctx, VSK_ERR_INVALID_INPUT, "null pointer");
   drain_stale_error("vsk_q4_decode_dev");
   VSK_TRY(decode(ctx, rows, out));
+  tl_mark(ctx, "q4_decode");
   VSK_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
   return VSK_OK;
 }
@@ -401,10 +403,11 @@ int32_t vsk_q4_product_dev(vsk_ctx* c, const vsk_q4_rows* rows, const void* x, i
   if ((reinterpret_cast<uintptr_t>(x) & (uintptr_t)(xs - 1)) || (reinterpret_cast<uintptr_t>(y) & (uintptr_t)(ys - 1)))
     return fail(ctx, VSK_ERR_INVALID_INPUT, "a pointer is not aligned to its element");
   drain_stale_error("vsk_q4_product_dev");
-  // 200 000 x 2 048, groups of 128 / of 32 with middles: five fp16 vectors take 75 / 130 us in whole numbers and 91 / 142 in 16 bits, six
-  // 99 / 175 and 91 / 143 (a third tile of digits).  fp32 vectors have no 16-bit form.
-  if (x_dtype == VSK_DTYPE_F32 || nq <= 5) VSK_TRY(q4_product_digits(ctx, *rows, x, x_dtype, nq, x_stride, y, y_dtype, y_stride));
+  // 200 000 x 2 048, groups of 128 / of 32 with middles: four fp16 vectors take 74 / 123 us in whole numbers and 91 / 143 in 16 bits, six
+  // 99 / 175 and 91 / 143 (they no longer fit two tiles of digits).  fp32 vectors have no 16-bit form.
+  if (x_dtype == VSK_DTYPE_F32 || nq <= 4) VSK_TRY(q4_product_digits(ctx, *rows, x, x_dtype, nq, x_stride, y, y_dtype, y_stride));
   else VSK_TRY(q4_product(ctx, *rows, x, x_dtype, nq, x_stride, y, y_dtype, y_stride));
+  tl_mark(ctx, "q4_product");
   VSK_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
   return VSK_OK;
 }

@@ -3,8 +3,8 @@
 // With one vector the call is bound by the bytes of the rows as long as unpacking keeps up with them: 6.5 TB/s are 46 codes per SM and
 // clock.  A code in the high half of a byte, its top bit turned, IS the signed byte 16 (code - 8): eight codes take three
 // instructions, a third of what any 16-bit form takes.  So x comes in whole numbers too.  Each vector is scaled by a power of two until
-// its largest element fills `digits` signed bytes (three for 16-bit types, four for fp32) and rounded there, by at most 2^-23 (2^-31) of that
-// element: an fp32 sum that contains it rounds by as much.  The bytes are columns of their own in m16n8k32 products; group sums are exact
+// its largest element fills four signed bytes and rounded there, by at most 2^-31 of that element: an fp32 sum that contains it rounds by
+// a hundred times as much.  The bytes are columns of their own in m16n8k32 products, a tile of eight holds two vectors; group sums are exact
 // whole numbers, become fp32 (a magic constant is the products' starting value: its difference is the number) and meet the scale there.
 // A vector with an infinity or a NaN has no such form: its products are taken one by one in fp32.
 //
@@ -26,6 +26,7 @@ namespace vsk {
 namespace {
 
 constexpr int kWarps = 8;
+constexpr int kDigits = 4;           // of a vector's numbers
 constexpr int kMagic = 0x4b400000;   // the bits of 1.5 2^23: that many more as a whole number is as much more as an fp32 number
 
 struct VectorInfo {
@@ -50,7 +51,7 @@ struct DigitArgs {
   int64_t x_stride;
   int x_dtype;
   int64_t nq;
-  int digits, per_launch;     // columns per vector; vectors per grid row
+  int per_launch;             // vectors per grid row
   void* y;
   int64_t y_stride;
   int y_dtype;
@@ -130,7 +131,7 @@ template <int DT>
 struct Shape {
   static constexpr int kStage = 32 * 64;
   static constexpr int kStages = DT == 4 ? 6 : 4;
-  static constexpr int kVectors = DT * 8 / 3;                // at most, with three digits
+  static constexpr int kVectors = DT * 8 / kDigits;
   static constexpr int kLine = 8 * DT + kVectors + 1;        // floats of a row of the epilogue's buffer: digits, then middles' share per vector
   static constexpr int kScales = 2 * 32 * 4;                 // two steps' scales
   static constexpr size_t kRing = (size_t)kWarps * kStages * kStage;
@@ -450,15 +451,16 @@ __global__ void __launch_bounds__(32 * kWarps, DT == 4 ? 1 : 2) q4_digits_kernel
     for (int q = wk; q < nq; q += team) {
       const int exponent = VSK_CHK(a.info + q0 + q)->exponent;
       float v = 0.f, m = 0.f;
-      for (int d = 0; d < a.digits; ++d) {   // the small digits first
+#pragma unroll
+      for (int d = 0; d < kDigits; ++d) {   // the small digits first
         float part = 0.f;
-        for (int w = 0; w < team; ++w) part += red[(w * 32 + lane) * S::kLine + q * a.digits + d];
+        for (int w = 0; w < team; ++w) part += red[(w * 32 + lane) * S::kLine + q * kDigits + d];
         v = fmaf(v, 1.f / 256.f, part);
       }
       if constexpr (MID)
         for (int w = 0; w < team; ++w) m += red[(w * 32 + lane) * S::kLine + 8 * DT + q];
-      // (the digits' numbers are 16 times the products, and the last one added counts 256^(digits - 1))
-      v = ldexpf(v, exponent + 8 * (a.digits - 1) - 4) + m;
+      // (the digits' numbers are 16 times the products, and the last one added counts 256^3)
+      v = ldexpf(v, exponent + 8 * (kDigits - 1) - 4) + m;
       if (row < a.n) {
         if (exponent == INT_MIN) v = plain_product(a, row, q0 + q);
         store_y(a, (q0 + q) * a.y_stride + row, v);
@@ -472,7 +474,7 @@ __global__ void __launch_bounds__(32 * kWarps, DT == 4 ? 1 : 2) q4_digits_kernel
 // thread; of vectors of up to 8 192 nothing is read twice.
 constexpr int kToDigits = 512, kKept = 2;
 template <typename X>
-__global__ void __launch_bounds__(kToDigits) q4_to_digits_kernel(const X* __restrict__ x, int64_t x_stride, int wide, int dim, int ksteps, int digits,
+__global__ void __launch_bounds__(kToDigits) q4_to_digits_kernel(const X* __restrict__ x, int64_t x_stride, int wide, int dim, int ksteps,
                                                                  int per_launch, int tiles, int group, uint2* __restrict__ frags,
                                                                  float* __restrict__ sums, int sum_stride, VectorInfo* __restrict__ info) {
   __shared__ float warp_top[kToDigits / 32];
@@ -530,30 +532,28 @@ __global__ void __launch_bounds__(kToDigits) q4_to_digits_kernel(const X* __rest
 #pragma unroll
   for (int w = 0; w < kToDigits / 32; ++w) top = fmaxf(top, warp_top[w]);
   const bool finite = wrong == 0;
-  // the largest power of two that keeps |top| within 127 256^(digits-1) + ... + 127
-  const float most = digits == 4 ? 2139062144.f - 128.f : 8355711.f;
+  // the largest power of two that keeps |top| within 127 256^3 + 127 256^2 + 127 256 + 127
   int shift = 0;
   if (finite && top > 0.f) {
-    shift = 8 * digits - 2 - ilogbf(top);      // top 2^shift in [2^(8 digits - 2), 2^(8 digits - 1))
-    if (ldexpf(top, shift) > most) --shift;
+    shift = 30 - ilogbf(top);      // top 2^shift in [2^30, 2^31)
+    if (ldexpf(top, shift) > 2139062016.f) --shift;
   }
   if (threadIdx.x == 0) info[q] = VectorInfo{finite ? -shift : INT_MIN};
   // a power of two beyond fp32's range is taken in two steps
   const float up0 = ldexpf(1.f, max(-126, min(127, shift))), up1 = ldexpf(1.f, shift - max(-126, min(127, shift)));
   const int64_t chunk = q / per_launch;
-  const int first_col = (int)(q % per_launch) * digits;
+  const int first_col = (int)(q % per_launch) * kDigits;
   auto put = [&](int p, const float (&v)[8]) {   // (whole warps together, for the sums)
     const int col = p * 8;
     const bool inside = p < ksteps * 16;
-    uint32_t even[4] = {}, odd[4] = {};
+    uint32_t even[kDigits] = {}, odd[kDigits] = {};
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       s += v[j];
       int n = __float2int_rn(v[j] * up0 * up1);
 #pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        if (d == digits) break;
+      for (int d = 0; d < kDigits; ++d) {
         const int low = (int)(int8_t)(n & 0xff);
         n = (n - low) >> 8;
         if (j & 1) odd[d] |= (uint32_t)(low & 0xff) << (8 * (j >> 1));
@@ -564,8 +564,7 @@ __global__ void __launch_bounds__(kToDigits) q4_to_digits_kernel(const X* __rest
     const int k = p >> 4, sub = group == 32 ? (p >> 2) & 3 : group == 64 ? ((p >> 2) & 2) | (p & 1) : p & 3;
     const int t = group == 32 ? p & 3 : group == 64 ? (p >> 1) & 3 : (p >> 2) & 3;
 #pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      if (d == digits) break;
+    for (int d = 0; d < kDigits; ++d) {
       const int c = first_col + d, lane = (c & 7) * 4 + t;
       // [chunk][kstep][tile][sub / 2][lane][sub & 1]
       const int64_t at = ((((chunk * ksteps + k) * tiles + (c >> 3)) * 2 + (sub >> 1)) * 32 + lane) * 2 + (sub & 1);
@@ -660,10 +659,8 @@ int32_t q4_product_digits(Ctx* ctx, const vsk_q4_rows& rows, const void* x, int3
   a.y = y;
   a.y_stride = y_stride;
   a.y_dtype = y_dtype;
-  a.digits = x_dtype == VSK_DTYPE_F32 ? 4 : 3;
-  const int64_t cols = nq * a.digits;
-  const int tiles = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
-  a.per_launch = 8 * tiles / a.digits;
+  const int tiles = nq <= 2 ? 1 : nq <= 4 ? 2 : 4;
+  a.per_launch = 8 * tiles / kDigits;
   const int64_t chunks = ceil_div(nq, a.per_launch);
   if (chunks > 65535) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "too many vectors");
   const size_t frag_bytes = (size_t)chunks * a.ksteps * tiles * 1024;
@@ -679,7 +676,7 @@ int32_t q4_product_digits(Ctx* ctx, const vsk_q4_rows& rows, const void* x, int3
   auto prepare = [&](auto* v) {
     using X = std::remove_const_t<std::remove_pointer_t<decltype(v)>>;
     const int wide = ((reinterpret_cast<uintptr_t>(v) | (uintptr_t)(x_stride * sizeof(X))) & 15) == 0;
-    q4_to_digits_kernel<X><<<(unsigned)nq, kToDigits, 0, ctx->stream>>>(v, x_stride, wide, a.dim, a.ksteps, a.digits, a.per_launch, tiles, a.group, (uint2*)p, sums,
+    q4_to_digits_kernel<X><<<(unsigned)nq, kToDigits, 0, ctx->stream>>>(v, x_stride, wide, a.dim, a.ksteps, a.per_launch, tiles, a.group, (uint2*)p, sums,
                                                                   a.sum_stride, info);
   };
   if (x_dtype == VSK_DTYPE_F32) prepare((const float*)x);
