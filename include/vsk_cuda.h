@@ -546,7 +546,7 @@ int32_t vsk_pq_index_add_dev(vsk_index* index, const uint8_t* codes, int64_t n);
  *               last column is 8.  Bytes behind a row's columns are neither read nor written.
  *   scales, middles   [n] rows of scale_stride fp16 numbers, one per group; encoding writes them dense (stride = groups)
  * Element types of the `void*` arguments: vsk_dtype.  Strides count elements, code_stride bytes.
- *   encode      rows[n][row_stride] -> codes, scales, middles (NULL with symmetric != 0)
+ *   encode      rows[n][row_stride] -> codes, scales, middles (NULL with symmetric != 0); what lies between the rows may be read
  *   decode      -> out[n][dim] fp32, each value rounded once
  *   product     y[q * y_stride + r] = sum over the columns of value(r, i) x[q * x_stride + i]: the scores of nq vectors
  *               against all rows, as a decoding step takes them from a projection or an output head, or a query from a store

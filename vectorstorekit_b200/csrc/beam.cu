@@ -505,8 +505,10 @@ int32_t select(Ctx* ctx, BeamArgs a) {
 }
 
 // ---- states ---------------------------------------------------------------------------------------------------------------------
-// A thread owns one vector of W bytes at one place of all the rows of a batch entry: it loads what every slot takes from its parent and only
-// then stores, so rows may change places in place, in any permutation.
+// A thread owns vectors of W bytes, each at one place of all the rows of a batch entry: it loads what every slot takes from its parent and only
+// then stores, so rows may change places in place, in any permutation.  Four such places per thread: a block's look at the parents and its
+// place in the list of states cost as much as moving 4 KB.
+constexpr int kPlaces = 4;
 constexpr int kStatesPerLaunch = 32;
 struct StateMove {
   const uint8_t* src;
@@ -514,7 +516,7 @@ struct StateMove {
   int64_t src_row, dst_row, src_outer, dst_outer;   // bytes between rows / between the outer parts of a row
   int64_t outer, inner;                             // outer parts, bytes of one
   int64_t step;                                     // bytes of a time step, 0: no time axis
-  int64_t first_block;
+  unsigned first_block, tiles;                      // blocks before this state's, blocks along one part
 };
 struct StateArgs {
   StateMove move[kStatesPerLaunch];
@@ -527,52 +529,59 @@ struct StateArgs {
 
 template <typename V, int SLOTS>
 __global__ void __launch_bounds__(256) reorder_kernel(const __grid_constant__ StateArgs a) {
+  constexpr int kAtOnce = SLOTS <= 8 ? 2 : 1;   // places under way
   __shared__ int from[kMaxBeams];
   __shared__ int moving, wrong;
   int s = 0;
-  while (s + 1 < a.count && (int64_t)blockIdx.x >= a.move[s + 1].first_block) ++s;
+  while (s + 1 < a.count && blockIdx.x >= a.move[s + 1].first_block) ++s;
   const StateMove& m = a.move[s];
-  const int64_t tiles = (m.inner + 256 * sizeof(V) - 1) / (256 * sizeof(V));
-  int64_t at = (int64_t)blockIdx.x - m.first_block;
-  const int64_t tile = at % tiles;
-  at /= tiles;
-  const int64_t part = at % m.outer, b = at / m.outer;
+  unsigned at = blockIdx.x - m.first_block;
+  const unsigned tile = at % m.tiles;
+  at /= m.tiles;
+  const int64_t part = at % (unsigned)m.outer, b = at / (unsigned)m.outer;   // (the host keeps their product below 2^31)
+  if (threadIdx.x == 0) moving = wrong = 0;
+  __syncthreads();
   int64_t live = m.inner;
   if (m.step && a.lengths) {
     const int64_t len = __ldg(a.lengths + b);
     live = len <= 0 ? 0 : len >= m.inner / m.step ? m.inner : len * m.step;
   }
-  if (threadIdx.x == 0) moving = wrong = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.beams; i += 256) {
+  if (threadIdx.x < a.beams) {
+    const int i = threadIdx.x;
     const int64_t p = __ldg(a.parents + b * a.beams + i);
-    const bool ok = p >= -1 && p < a.beams;
-    from[i] = ok ? (int)p : -1;
+    const bool ok = p >= -1 && p < a.beams, moves = ok && p >= 0 && (p != i || m.src != m.dst);
+    from[i] = moves ? (int)p : -1;
     if (!ok) wrong = 1;
-    if (ok && p >= 0 && (p != i || m.src != m.dst)) moving = 1;
+    if (moves) moving = 1;
   }
   __syncthreads();
   if (wrong) {   // every block of this batch entry sees it: none of its rows moves
     if (threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.bad) = 1;
     return;
   }
-  const int64_t off = (tile * 256 + threadIdx.x) * (int64_t)sizeof(V);
-  if (!moving || off >= live) return;
-  const bool here = m.src == m.dst;
-  const uint8_t* src = m.src + b * a.beams * m.src_row + part * m.src_outer + off;
-  uint8_t* dst = m.dst + b * a.beams * m.dst_row + part * m.dst_outer + off;
-  // in place, SLOTS >= beams: everything is loaded before anything is stored
-  for (int i0 = 0; i0 < a.beams; i0 += SLOTS) {
-    V v[SLOTS];
+  if (!moving) return;
+  const uint8_t* const src = m.src + b * a.beams * m.src_row + part * m.src_outer;
+  uint8_t* const dst = m.dst + b * a.beams * m.dst_row + part * m.dst_outer;
+  const int64_t first = ((int64_t)tile * (256 * kPlaces) + threadIdx.x) * (int64_t)sizeof(V);
+#pragma unroll 1
+  for (int place = 0; place < kPlaces; place += kAtOnce) {
+    int64_t off[kAtOnce];
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i) {
-      const int slot = i0 + i;
-      if (slot < a.beams && from[slot] >= 0 && !(here && from[slot] == slot)) v[i] = *VSK_CHK(reinterpret_cast<const V*>(src + from[slot] * m.src_row));
-    }
+    for (int u = 0; u < kAtOnce; ++u) off[u] = first + (place + u) * (256 * (int64_t)sizeof(V));
+    if (off[0] >= live) return;
+    // in place, SLOTS >= beams: everything is loaded before anything is stored
+    for (int i0 = 0; i0 < a.beams; i0 += SLOTS) {
+      V v[kAtOnce][SLOTS];
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i) {
-      const int slot = i0 + i;
-      if (slot < a.beams && from[slot] >= 0 && !(here && from[slot] == slot)) *VSK_CHK_W(reinterpret_cast<V*>(dst + slot * m.dst_row)) = v[i];
+      for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i)
+          if (off[u] < live && i0 + i < a.beams && from[i0 + i] >= 0) v[u][i] = *VSK_CHK(reinterpret_cast<const V*>(src + from[i0 + i] * m.src_row + off[u]));
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i)
+          if (off[u] < live && i0 + i < a.beams && from[i0 + i] >= 0) *VSK_CHK_W(reinterpret_cast<V*>(dst + (i0 + i) * m.dst_row + off[u])) = v[u][i];
     }
   }
 }
@@ -590,10 +599,13 @@ int32_t reorder(Ctx* ctx, StateArgs& a, bool in_place) {
   int64_t blocks = 0;
   for (int i = 0; i < a.count; ++i) {
     StateMove& m = a.move[i];
-    m.first_block = blocks;
-    blocks += a.batch * m.outer * ceil_div(m.inner, 256 * (int64_t)sizeof(V));
+    const int64_t tiles = ceil_div(m.inner, 256 * kPlaces * (int64_t)sizeof(V));
+    if (tiles > 0x7fffffffLL || m.outer > 0x7fffffffLL || a.batch * m.outer > 0x7fffffffLL / tiles || blocks + a.batch * m.outer * tiles > 0x7fffffffLL)
+      return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "the states are too large for one call");
+    m.first_block = (unsigned)blocks;
+    m.tiles = (unsigned)tiles;
+    blocks += a.batch * m.outer * tiles;
   }
-  if (blocks > 0x7fffffffLL) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "the states are too large for one call");
   if (!in_place || a.beams <= 8) reorder_kernel<V, 8><<<(unsigned)blocks, 256, 0, ctx->stream>>>(a);
   else if (a.beams <= 16) reorder_kernel<V, 16><<<(unsigned)blocks, 256, 0, ctx->stream>>>(a);
   else if (a.beams <= 32) reorder_kernel<V, 32><<<(unsigned)blocks, 256, 0, ctx->stream>>>(a);

@@ -59,9 +59,9 @@ __device__ __forceinline__ unsigned nearest_codes(const float (&x)[8], float mid
   return c;
 }
 
-template <typename T, bool SYMMETRIC>
+template <typename T, bool SYMMETRIC, bool WIDE>
 __global__ void __launch_bounds__(256) q4_encode_kernel(const T* __restrict__ rows, int64_t n, int dim, int64_t row_stride, int group,
-                                                        int groups, int lanes, int columns, int wide, uint8_t* __restrict__ codes,
+                                                        int groups, int lanes, int columns, uint8_t* __restrict__ codes,
                                                         int64_t code_stride, __half* __restrict__ scales,
                                                         __half* __restrict__ middles) {
   const int lane = threadIdx.x & (lanes - 1), per_block = 256 / lanes;
@@ -73,9 +73,35 @@ __global__ void __launch_bounds__(256) q4_encode_kernel(const T* __restrict__ ro
   const int first = blockIdx.y * columns, end = min(dim, first + columns), stride = 8 * lanes;
   const int group_shift = group == 32 ? 5 : group == 64 ? 6 : 7;
 
+  // Rows that do not begin at 16-byte boundaries: aligned vectors around the lane's eight columns, shifted together.  They may reach into a
+  // neighbouring row, never out of the rows' memory.
+  const int off = (int)(reinterpret_cast<uintptr_t>(src) & 15);
+  const uint8_t* const begin = reinterpret_cast<const uint8_t*>(rows);
+  const uint8_t* const finish = reinterpret_cast<const uint8_t*>(rows + (n - 1) * row_stride + dim);
   auto load = [&](int col, float (&v)[8]) {
     const int have = inside ? min(8, end - col) : 0;
-    if (wide && have == 8) {
+    constexpr int kWords = 2 * (int)sizeof(T);   // of eight columns
+    const uint8_t* const from = reinterpret_cast<const uint8_t*>(src + col) - off;
+    if (!WIDE && have == 8 && from >= begin && from + 4 * kWords + 16 <= finish) {
+      uint32_t w[kWords + 4];
+#pragma unroll
+      for (int i = 0; i < kWords + 4; i += 4) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(from + 4 * i));
+        w[i] = u.x; w[i + 1] = u.y; w[i + 2] = u.z; w[i + 3] = u.w;
+      }
+#pragma unroll
+      for (int i = 0; i < kWords + 2; ++i) w[i] = (off & 8) ? w[i + 2] : w[i];
+#pragma unroll
+      for (int i = 0; i < kWords + 1; ++i) w[i] = (off & 4) ? w[i + 1] : w[i];
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 8 * (off & 2));
+      }
+      T h[8];
+      memcpy(h, w, sizeof(h));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = to_float<T>(h[j]);
+    } else if (WIDE && have == 8) {
       if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int j = 0; j < 8; j += 4) {
@@ -152,8 +178,10 @@ __global__ void __launch_bounds__(256) q4_decode_kernel(const uint8_t* __restric
                                                         const __half* __restrict__ scales, const __half* __restrict__ middles,
                                                         int64_t scale_stride, int64_t n, int dim, int group_shift, int lanes, int columns,
                                                         float* __restrict__ out) {
+  __shared__ __align__(16) float staged[8][256];   // what a warp writes at once, where rows do not begin at 16-byte boundaries
   const int64_t row = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
-  if (row >= n) return;
+  const bool inside = row < n;   // (whole warps walk together)
+  const bool apart = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(4 * dim)) & 15) != 0;
   const uint8_t* const line = codes + row * code_stride;
   const __half* const s_line = scales + row * scale_stride;
   const __half* const m_line = middles + row * scale_stride;
@@ -164,7 +192,7 @@ __global__ void __launch_bounds__(256) q4_decode_kernel(const uint8_t* __restric
   __half s[kDecodeSteps], m[kDecodeSteps];
 #pragma unroll
   for (int i = 0; i < kDecodeSteps; ++i) {
-    const int col = first + i * lanes * 8, have = min(8, end - col);
+    const int col = first + i * lanes * 8, have = inside ? min(8, end - col) : 0;
     w[i] = 0;
     s[i] = m[i] = __half(0.f);
     if (have <= 0) continue;
@@ -179,8 +207,9 @@ __global__ void __launch_bounds__(256) q4_decode_kernel(const uint8_t* __restric
   }
 #pragma unroll
   for (int i = 0; i < kDecodeSteps; ++i) {
-    const int col = first + i * lanes * 8, have = min(8, end - col);
-    if (have <= 0) continue;
+    const int col = first + i * lanes * 8, have = inside ? min(8, end - col) : 0;
+    const int base = blockIdx.y * columns + i * lanes * 8;   // of this step, the same for the whole warp
+    if (base >= end) break;
     const float scale = __half2float(s[i]), middle = __half2float(m[i]);
     float v[8];
 #pragma unroll
@@ -189,11 +218,22 @@ __global__ void __launch_bounds__(256) q4_decode_kernel(const uint8_t* __restric
       if (middles) v[j] = __fadd_rn(v[j], middle);
     }
     float* dst = to + col;
-    if (have == 8 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+    if (have == 8 && !apart) {
       *VSK_CHK_W(reinterpret_cast<float4*>(dst)) = make_float4(v[0], v[1], v[2], v[3]);
       *VSK_CHK_W(reinterpret_cast<float4*>(dst + 4)) = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
+    } else if (!apart) {
       for (int j = 0; j < have; ++j) *VSK_CHK_W(dst + j) = v[j];
+    } else {
+      // A warp's rows of this step follow one another in memory: a part of one row, or (short rows) several whole ones.
+      const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, span = min(lanes * 8, end - base);
+      float* const at = staged[warp] + (lane / lanes) * span + (col - base);
+      for (int j = 0; j < have; ++j) at[j] = v[j];
+      __syncwarp();
+      const int64_t row0 = row - lane / lanes;   // the warp's first
+      const int rows = (int)min((int64_t)(32 / lanes), max((int64_t)0, n - row0));
+      float* const all = out + row0 * dim + base;
+      for (int e = lane; e < rows * span; e += 32) *VSK_CHK_W(all + e) = staged[warp][e];
+      __syncwarp();
     }
   }
 }
@@ -240,8 +280,9 @@ int32_t encode(Ctx* ctx, const void* rows, int32_t dtype, int64_t n, int32_t dim
   auto go = [&](auto* x) {
     using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
     const dim3 grid((unsigned)blocks, (unsigned)along);
-    if (symmetric) q4_encode_kernel<T, true><<<grid, 256, 0, ctx->stream>>>(x, n, dim, row_stride, group, groups, lanes, columns, wide, codes, code_stride, (__half*)scales, nullptr);
-    else q4_encode_kernel<T, false><<<grid, 256, 0, ctx->stream>>>(x, n, dim, row_stride, group, groups, lanes, columns, wide, codes, code_stride, (__half*)scales, (__half*)middles);
+    auto kernel = symmetric ? (wide ? q4_encode_kernel<T, true, true> : q4_encode_kernel<T, true, false>)
+                            : (wide ? q4_encode_kernel<T, false, true> : q4_encode_kernel<T, false, false>);
+    kernel<<<grid, 256, 0, ctx->stream>>>(x, n, dim, row_stride, group, groups, lanes, columns, codes, code_stride, (__half*)scales, (__half*)middles);
   };
   if (dtype == VSK_DTYPE_F32) go((const float*)rows);
   else if (dtype == VSK_DTYPE_F16) go((const __half*)rows);

@@ -416,9 +416,7 @@ int32_t launch(Ctx* ctx, ProductArgs a) {
   const int64_t slots = (int64_t)ctx->prop.multiProcessorCount * resident_blocks(ctx, kernel, 32 * kWarps, S::kShared) * kWarps;
   const int64_t tiles = ceil_div(a.n, 32);
   if (tiles > 1 << 30) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "too many rows in one call");
-  // few rows: warps of a block share a tile's columns until the device is full
-  a.team = 1;
-  while (a.team < kWarps && 2 * a.team <= a.ksteps && tiles * a.team * chunks < slots) a.team *= 2;
+  a.team = q4_team(tiles, a.ksteps, std::max<int64_t>(1, slots / chunks), kWarps);
   const int64_t blocks = std::min(ceil_div(tiles, kWarps / a.team), std::max<int64_t>(1, slots / kWarps / chunks));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)blocks, (unsigned)chunks);

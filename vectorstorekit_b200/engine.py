@@ -219,6 +219,30 @@ def _row_stride(t) -> int:
     return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
 
 
+def _state_layout(t, o, rows, axis, timed):
+    """The fields of ``vsk_state`` behind the two addresses."""
+    shape = t.shape
+    if len(shape) == 0 or shape[0] != rows:
+        raise DimensionMismatch(f"a state must have {rows} rows, got {tuple(shape)}")
+    if o.shape != shape or o.dtype != t.dtype:
+        raise DimensionMismatch("a result must have its state's shape and type")
+    if t.numel() == 0:
+        raise EmptyInput("a state is empty")
+    if axis is not None and not 1 <= axis < len(shape):
+        raise InvalidInput(f"time axis {axis} of a state with {len(shape)} dimensions")
+    e = t.element_size()
+    if t.is_contiguous() and o.is_contiguous():
+        row = per_step = t.numel() // rows
+        for n in shape[1:axis + 1] if timed else ():
+            per_step //= n
+        steps = shape[axis] if timed else 1
+        part = steps * per_step
+        return row * e, row * e, part * e, part * e, row // part, steps, per_step * e, 1 if timed else 0, 0
+    outer, inner, steps, per_step, src_outer, dst_outer = _row_parts(t, o, axis if timed else None)
+    src_row, dst_row = ((x.stride(0) if rows > 1 else inner * outer) * e for x in (t, o))
+    return src_row, dst_row, src_outer * e, dst_outer * e, outer, steps, per_step * e, 1 if timed else 0, 0
+
+
 def _row_parts(t, o, axis):
     """How a row of a state is laid out: ``outer`` parts of ``steps * per_step`` contiguous elements, in the state and its result.
     -> (outer, elements of a part, steps, per_step, distance of parts in the state, in the result)"""
@@ -557,33 +581,15 @@ class CUDAAccelerationEngine:
             raise DimensionMismatch("one time axis and one result per state")
         rows = b * w
         moves = C.create_string_buffer(_lib.STATE.size * len(states))
+        last = layout = None
         for i, (t, o, axis) in enumerate(zip(states, results, axes)):
             if not _is_dev(t) or not _is_dev(o):
                 raise InvalidInput("reorderStates takes CUDA tensors")
-            shape = t.shape
-            if len(shape) == 0 or shape[0] != rows:
-                raise DimensionMismatch(f"a state must have {rows} rows, got {tuple(shape)}")
-            if o is not t and (o.shape != shape or o.dtype != t.dtype):
-                raise DimensionMismatch("a result must have its state's shape and type")
-            if t.numel() == 0:
-                raise EmptyInput("a state is empty")
-            if axis is not None and not 1 <= axis < len(shape):
-                raise InvalidInput(f"time axis {axis} of a state with {len(shape)} dimensions")
-            timed = axis is not None and lengths is not None
-            e = t.element_size()
-            if t.is_contiguous() and (o is t or o.is_contiguous()):
-                src_row = dst_row = t.numel() // rows
-                per_step = src_row
-                for n in shape[1:axis + 1] if timed else ():
-                    per_step //= n
-                steps = shape[axis] if timed else 1
-                src_outer = dst_outer = steps * per_step
-                outer = src_row // src_outer
-            else:
-                outer, inner, steps, per_step, src_outer, dst_outer = _row_parts(t, o, axis if timed else None)
-                src_row, dst_row = (x.stride(0) if rows > 1 else inner * outer for x in (t, o))
-            _lib.STATE.pack_into(moves, i * _lib.STATE.size, t.data_ptr(), o.data_ptr(), src_row * e, dst_row * e, src_outer * e, dst_outer * e,
-                                 outer, steps, per_step * e, 1 if timed else 0, 0)
+            own = t is o
+            this = (t.shape, t.stride(), t.dtype, axis, None if own else (o.shape, o.stride(), o.dtype))
+            if this != last:   # (the layers of a model have the same layout)
+                layout, last = _state_layout(t, o, rows, axis, axis is not None and lengths is not None), this
+            _lib.STATE.pack_into(moves, i * _lib.STATE.size, t.data_ptr(), o.data_ptr(), *layout)
         parents = parents.contiguous()
         lengths = None if lengths is None else lengths.contiguous()
         pp, pl, *_ = _device_pointers(self.dev, parents, lengths, *states, *(results if out is not None else ()))
