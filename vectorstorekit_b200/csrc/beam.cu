@@ -22,7 +22,9 @@ constexpr int kMaxBeams = 64;
 constexpr int kMaxBeamK = 128;
 constexpr int kListed = 1024;     // candidates that a selection can order at once
 constexpr int kChosen = 512;      // pieces that it reads again
-constexpr int kSmall = 8192;      // candidates of a batch entry that are staged in shared memory
+// Candidates of a batch entry that are staged in shared memory.  1 000 entries of 4 x 400: 49 us staged, 69 in pieces; 100 of 4 x 500: 46
+// and 42; 500 of 8 x 1 000: 76 and 60 (the calls, normalised fp32).
+constexpr int kSmall = 2048;
 
 struct BeamArgs {
   const void* logits;
@@ -64,8 +66,8 @@ template <> __device__ __forceinline__ float lowest<float>() { return -CUDART_IN
 template <> __device__ __forceinline__ __half lowest<__half>() { return __ushort_as_half(0xfc00); }
 template <> __device__ __forceinline__ __nv_bfloat16 lowest<__nv_bfloat16>() { return __ushort_as_bfloat16(0xff80); }
 
-// A warp takes a.per_warp pieces of a row one after the other, the next one's loads under way.  32 x 8 x 131 072 bf16 logits (67 MB): bound by
-// the instructions of a logit (convert, maximum, convert, subtract, multiply, power, add).
+// A warp takes a.per_warp pieces of a row one after the other, the next one's loads under way.  32 x 8 x 131 072 bf16 logits (67 MB): 20 us,
+// 3.3 TB/s, issue slots 61 % busy: bound by the instructions of a logit (convert, maximum, convert, subtract, multiply, power, add).
 template <typename T>
 __global__ void __launch_bounds__(256) beam_pieces_kernel(const BeamArgs a) {
   constexpr int kVec = 16 / sizeof(T), kLoads = kPiece / (32 * kVec);
@@ -247,7 +249,8 @@ __device__ unsigned bound_of(unsigned own, int k, unsigned* shared) {
   return lo;
 }
 
-// One block per batch entry.  SMALL: the candidates are staged in shared memory; otherwise their pieces are ranked first.
+// One block per batch entry.  SMALL: the candidates are staged in shared memory; otherwise their pieces are ranked first.  A chain of short
+// dependent steps, bound by their latency: 12 us for one entry of 4 x 32 768, 19 for 32 of 8 x 131 072, 15 for 1 000 of 8 x 100 (SMALL).
 template <typename T, int THREADS, bool SMALL>
 __global__ void __launch_bounds__(THREADS) beam_choose_kernel(const BeamArgs a) {
   __shared__ Key list[kListed];
@@ -460,13 +463,8 @@ template <typename T>
 int32_t select(Ctx* ctx, BeamArgs a) {
   const int64_t candidates = a.beams * a.vocab;
   if (candidates <= kSmall) {
-    const size_t shared = (size_t)candidates * sizeof(float);
-    if (candidates <= 2048) beam_choose_kernel<T, 128, true><<<(unsigned)a.batch, 128, shared, ctx->stream>>>(a);
-    else {
-      // (the list and the candidates together pass 48 KB)
-      VSK_CUDA(ctx, opt_in_shared(ctx, beam_choose_kernel<T, 512, true>, kSmall * sizeof(float)));
-      beam_choose_kernel<T, 512, true><<<(unsigned)a.batch, 512, shared, ctx->stream>>>(a);
-    }
+    // 1 000 entries of 8 x 100 and 4 x 400: 46 and 49 us with four warps to an entry, 60 and 57 with sixteen; 100 of 4 x 500: 46 and 40
+    beam_choose_kernel<T, 128, true><<<(unsigned)a.batch, 128, (size_t)candidates * sizeof(float), ctx->stream>>>(a);
     ctx->stats.kernel_launches++;
     VSK_CUDA(ctx, cudaGetLastError());
     return VSK_OK;
@@ -474,13 +472,14 @@ int32_t select(Ctx* ctx, BeamArgs a) {
   constexpr int kParts = kPiece * (int)sizeof(T) / 512;
   a.pieces = (int)ceil_div(a.vocab + 16 / (int)sizeof(T) - 1, kPiece);
   const int64_t items = a.batch * a.beams * a.pieces;
-  // parts of pieces where whole ones are few against k: the bound then leaves fewer candidates
+  // Parts of pieces where whole ones are few against k: the bound then leaves fewer candidates.  Four rows of 50 000, k = 64: 48 us with
+  // parts, 180 without (more candidates than a list orders); 64 beams of 65 536, k = 128: 119 and 93.
   const bool parts = (int64_t)a.beams * a.pieces < 16 * (int64_t)a.k;
   void* p;
   VSK_TRY(scratch(ctx, SLOT_BEAM, (size_t)items * (sizeof(float2) + (parts ? kParts * sizeof(float) : 0)), &p));
   a.stats = (float2*)p;
   a.parts = parts ? (float*)(a.stats + items) : nullptr;
-  // as many pieces per warp as leave two rounds of warps
+  // as many pieces per warp as leave two rounds of warps (32 x 8 x 131 072 fp32: 84 us, one piece each: 87)
   a.per_warp = (int)std::max<int64_t>(1, std::min<int64_t>(8, items / ((int64_t)ctx->prop.multiProcessorCount * 64)));
   for (int64_t f = 0; f < a.batch; f += 65535) {
     a.first_batch = f;
@@ -507,7 +506,8 @@ int32_t select(Ctx* ctx, BeamArgs a) {
 // ---- states ---------------------------------------------------------------------------------------------------------------------
 // A thread owns vectors of W bytes, each at one place of all the rows of a batch entry: it loads what every slot takes from its parent and only
 // then stores, so rows may change places in place, in any permutation.  Four such places per thread: a block's look at the parents and its
-// place in the list of states cost as much as moving 4 KB.
+// place in the list of states cost as much as moving 4 KB (27 states of 3 x 8 x 766 x 128 fp32: 160 -> 131 us).  Eight states of
+// 64 x 8 x 1 024 x 128 bf16 into a second set: 205 us for 1.15 GB read and written, 5.6 TB/s, 0.86 of a copy's rate.
 constexpr int kPlaces = 4;
 constexpr int kStatesPerLaunch = 32;
 struct StateMove {

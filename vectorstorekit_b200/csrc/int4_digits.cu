@@ -15,6 +15,10 @@
 //           The product kernel is launched with it and has its first codes under way before it waits for it.
 //   scales  asked for by the row's lane two steps ahead, handed to the fragments' lanes as fp32 numbers in shared memory
 //   middles a row's middles times the vectors' group sums, in the row's lane
+//
+// 1 000 000 x 768, groups of 32 with middles, one fp32 vector (480 MB): 96 us, 5.0 TB/s, 0.77 of a copy's rate, issue slots 65 % busy (150
+// instructions for 16 rows x 128 columns: 24 unpack, 40 scale and sum the four groups).  200 000 x 2 048, groups of 128, one fp16 vector:
+// 43 us, 4.9 TB/s.  16-bit products of the same shape took three times as long, 32 rows with digits on the left side 1.2 times.
 #include <cuda_bf16.h>
 
 #include <algorithm>

@@ -8,6 +8,8 @@
 //   FlatIndex, IVFIndex            VectorStore.search / IVFIndex.train/insert/search,
 //                                  API/VectorStore.swift:271-318, Indexes/IVFIndex.swift:80-202,397-446
 //   ScalarQuantizer                Quantization/ScalarQuantizer.swift (int8)
+//   Int4Quantizer                  the next step below it: four bits, a scale per group of columns
+//   selectBeams, reorderStates     a beam search's step (device memory)
 // Errors are thrown as exceptions named after MetalComputeError / IVFError cases.
 #pragma once
 #include <algorithm>
@@ -338,6 +340,69 @@ class ScalarQuantizer {
   std::shared_ptr<CUDAComputeDevice> dev_;
   bool per_dim_;
 };
+
+// Rows in four bits with an fp16 scale, and without `symmetric` an fp16 middle, per group of 32, 64 or 128 columns (vsk_cuda.h has the
+// format).  Host arrays for the codec, device memory for the products.
+class Int4Quantizer {
+ public:
+  struct Rows {
+    std::vector<uint8_t> codes;               // [n][(dim + 1) / 2]
+    std::vector<uint16_t> scales, middles;    // fp16 [n][groups]; middles empty: symmetric
+  };
+  Int4Quantizer(std::shared_ptr<CUDAComputeDevice> dev, int32_t groupSize = 64, bool symmetric = true)
+      : dev_(std::move(dev)), group_(groupSize), symmetric_(symmetric) {}
+  Rows quantizeBatch(const float* rows, int64_t n, int32_t dim) const {
+    Rows r;
+    const int64_t per_row = group_ > 0 ? (dim + (int64_t)group_ - 1) / group_ : 0;
+    r.codes.resize((size_t)std::max<int64_t>(n, 0) * (((size_t)std::max(dim, 0) + 1) / 2));
+    r.scales.resize((size_t)std::max<int64_t>(n, 0) * (size_t)std::max<int64_t>(per_row, 0));
+    if (!symmetric_) r.middles.resize(r.scales.size());
+    check(vsk_q4_encode(dev_->ctx(), rows, n, dim, group_, symmetric_ ? 1 : 0, r.codes.data(), ((int64_t)dim + 1) / 2, r.scales.data(),
+                        symmetric_ ? nullptr : r.middles.data()), dev_->ctx());
+    return r;
+  }
+  std::vector<float> dequantizeBatch(const Rows& r, int64_t n, int32_t dim) const {
+    std::vector<float> out((size_t)std::max<int64_t>(n, 0) * (size_t)std::max(dim, 0));
+    const vsk_q4_rows d = descriptor(r.codes.data(), r.scales.data(), symmetric_ ? nullptr : r.middles.data(), n, dim);
+    check(vsk_q4_decode(dev_->ctx(), &d, out.data()), dev_->ctx());
+    return out;
+  }
+  // y[q * n + r] = sum over columns of (value of row r) x[q * dim + column], all of it device memory with dense rows.
+  void product(const uint8_t* codes, const void* scales, const void* middles, int64_t n, int32_t dim, const void* x, vsk_dtype xType,
+               int64_t nq, void* y, vsk_dtype yType) const {
+    const vsk_q4_rows d = descriptor(codes, scales, middles, n, dim);
+    check(vsk_q4_product_dev(dev_->ctx(), &d, x, xType, nq, dim, y, yType, n), dev_->ctx());
+  }
+ private:
+  vsk_q4_rows descriptor(const uint8_t* codes, const void* scales, const void* middles, int64_t n, int32_t dim) const {
+    vsk_q4_rows d{};
+    d.codes = codes;
+    d.scales = scales;
+    d.middles = middles;
+    d.code_stride = ((int64_t)dim + 1) / 2;
+    d.scale_stride = group_ > 0 ? (dim + (int64_t)group_ - 1) / group_ : 0;
+    d.n = n;
+    d.dim = dim;
+    d.group = group_;
+    return d;
+  }
+  std::shared_ptr<CUDAComputeDevice> dev_;
+  int32_t group_;
+  bool symmetric_;
+};
+
+// The k best (beam, token) continuations of each batch entry over dense logits [batch][beams][vocab]; device memory (vsk_beam_select_dev).
+inline void selectBeams(CUDAComputeDevice& dev, const void* logits, vsk_dtype type, int64_t batch, int32_t beams, int64_t vocab,
+                        const float* scores, int32_t k, float* outScores, int64_t* outBeams, int64_t* outTokens, bool normalize = true,
+                        const uint8_t* finished = nullptr, int64_t endToken = 0) {
+  check(vsk_beam_select_dev(dev.ctx(), logits, type, batch, beams, vocab, beams * vocab, vocab, scores, finished, endToken, normalize ? 1 : 0, k,
+                            outScores, outBeams, outTokens), dev.ctx());
+}
+// The beams' states moved after their parents (vsk_reorder_states_dev).
+inline void reorderStates(CUDAComputeDevice& dev, const std::vector<vsk_state>& states, int64_t batch, int32_t beams, const int64_t* parents,
+                          const int64_t* lengths = nullptr) {
+  check(vsk_reorder_states_dev(dev.ctx(), states.data(), (int32_t)states.size(), batch, beams, parents, lengths), dev.ctx());
+}
 
 // ProductQuantizer (Quantization/ProductQuantizer.swift) with ProductQuantizationConfig's fields; codes are one byte
 // per segment, so codeSize is at most 8.
