@@ -587,7 +587,7 @@ int32_t vsk_q4_product_dev(vsk_ctx* ctx, const vsk_q4_rows* rows, const void* x,
  *               logits are not read
  *   out         [batch][k] totals rounded to fp32, descending, with their beams and tokens; places without a candidate have
  *               score -inf, beam -1, token -1
- * At most 64 beams, k at most 128, vocabulary and batch below 2^31. */
+ * At most 64 beams, k at most 128, vocabulary and batch below 2^31.  No output overlaps an input. */
 int32_t vsk_beam_select_dev(vsk_ctx* ctx, const void* logits, int32_t dtype, int64_t batch, int32_t beams, int64_t vocab,
                             int64_t batch_stride, int64_t beam_stride, const float* scores, const uint8_t* finished,
                             int64_t end_token, int32_t normalize, int32_t k, float* out_scores, int64_t* out_beams,
@@ -597,7 +597,8 @@ int32_t vsk_beam_select_dev(vsk_ctx* ctx, const void* logits, int32_t dtype, int
  * same strides): in place, in any permutation.  Otherwise dst must not overlap any src, and no two states the same
  * memory.  A row is `outer` parts of steps * step_bytes contiguous bytes.  timed != 0: steps are time steps, and only the
  * first lengths[b] of them move (lengths NULL: all); the bytes behind are left as they are.
- * A parent outside [-1, beams) leaves all states of its batch entry as they are and returns VSK_ERR_INVALID_INPUT. */
+ * A parent outside [-1, beams) leaves all states of its batch entry as they are and returns VSK_ERR_INVALID_INPUT.
+ * parents and lengths are read throughout the call: memory between a dst's first and last byte is refused for them. */
 typedef struct vsk_state {
   const void* src;
   void* dst;

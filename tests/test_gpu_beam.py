@@ -270,6 +270,65 @@ def test_beam_refusals(engine):
             engine.reorderStates(**a)
 
 
+def test_a_refused_state_leaves_the_others_of_its_call_alone(engine):
+    """A state of more parts than a launch has blocks (2^31, of one byte), beside one that could move: nothing moves."""
+    import torch
+    from vectorstorekit_b200 import _lib
+    a = torch.arange(2 * 64, dtype=torch.uint8, device="cuda").reshape(2, 64)
+    before, other = a.clone(), torch.zeros(64, dtype=torch.uint8, device="cuda")
+    parents = torch.tensor([[1, 0]], device="cuda")
+    good = _lib.STATE.pack(a.data_ptr(), a.data_ptr(), 64, 64, 0, 0, 1, 1, 64, 0, 0)
+    call = lambda states, p: engine._lib.vsk_reorder_states_dev(engine.dev._h, b"".join(states), len(states), 1, 2, C.c_void_p(p), None)
+    large = _lib.STATE.pack(other.data_ptr(), other.data_ptr(), 1, 1, 1, 1, 1 << 31, 1, 1, 0, 0)
+    assert call([good, large], parents.data_ptr()) == 4 and call([good], parents.data_ptr() + 4) == 7
+    assert call([good], a.data_ptr() + 16) == 7   # parents in the state
+    assert torch.equal(a, before)
+    assert call([good], parents.data_ptr()) == 0
+    assert torch.equal(a, before.flip(0))
+
+
+def test_two_contexts_at_once_and_a_stream_of_the_callers(engine):
+    """Workspaces belong to a context: steps of two threads do not disturb each other.  Inputs still being made on another stream are waited for."""
+    import threading
+
+    import torch
+    import vectorstorekit_b200 as vsk
+    gen = torch.Generator().manual_seed(5)
+    inputs = []
+    for vocab, dim, w in ((5003, 320, 4), (2000, 1030, 6)):
+        rows, x = torch.randn((vocab, dim), generator=gen).cuda(), torch.randn((w, dim), generator=gen).half().cuda()
+        inputs.append((rows, x, torch.randn((1, w), generator=gen).cuda(), torch.randn((w, 3, 50, 8), generator=gen).cuda()))
+
+    def step(e, rows, x, scores, state):
+        q = vsk.Int4Quantizer(e.dev, 64)
+        logits = q.product(x, *q.quantizeBatch(rows), out_dtype=torch.float32)
+        got = e.selectBeams(logits[None], scores, x.shape[0])
+        out = [torch.empty_like(state)]
+        e.reorderStates([state], got[1], out=out)
+        return [logits, *got, *out]
+
+    want = [step(engine, *i) for i in inputs]
+    other = vsk.CUDAAccelerationEngine(vsk.CUDAComputeDevice(0))
+    wrong, done = [], []
+
+    def repeat(e, i):
+        torch.cuda.set_device(0)
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                fresh = [t.clone() for t in inputs[i]]   # (made on this thread's stream)
+                wrong.extend(j for j, (a, b) in enumerate(zip(step(e, *fresh), want[i])) if not torch.equal(a, b))
+                done.append(i)
+
+    threads = [threading.Thread(target=repeat, args=a) for a in ((engine, 0), (other, 1))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    other.dev.close()
+    assert wrong == [] and len(done) == 40
+
+
 def test_a_beam_search_with_an_output_head_in_four_bits(engine):
     """Head -> selection -> states, six steps, beams that finish on the way: the same sequences as in 64 bits."""
     import torch

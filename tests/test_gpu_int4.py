@@ -298,6 +298,7 @@ def test_int4_refusals(dev):
     assert lib.vsk_q4_product_dev(h, None, p(x), 0, 4, 64, p(y), 0, 4) == 7
     assert lib.vsk_q4_product_dev(None, C.byref(r), p(x), 0, 4, 64, p(y), 0, 4) == 7
     assert lib.vsk_q4_decode_dev(h, C.byref(r), None) == 7
+    assert lib.vsk_q4_decode_dev(h, C.byref(r), C.c_void_p(y.data_ptr() + 2)) == 7
     assert lib.vsk_q4_encode_dev(h, p(x), 0, 4, 64, 64, 32, 0, p(codes), 32, p(scales), None) == 7      # middles missing
     assert lib.vsk_q4_encode_dev(h, p(x), 0, 4, 64, 63, 32, 1, p(codes), 32, p(scales), None) == 4
     assert lib.vsk_q4_encode_dev(h, p(x), 0, 4, 64, 64, 32, 1, p(codes), 31, p(scales), None) == 4

@@ -67,3 +67,32 @@ def test_the_plain_codec_is_within_half_a_step(symmetric):
     assert np.all(np.abs(plain.values(codes, scales, middles, 32) - x) <= s / 2 + slack)
     assert codes.min() >= 0 and codes.max() <= 15
     assert plain.pack(codes[:, :3])[0, 1] >> 4 == 8
+
+
+def test_cpp_quantiser_refuses_codes_of_other_sizes(tmp_path):
+    """Rows whose vectors do not have the size that the call states are not read behind their ends: no device is asked."""
+    import os
+    import subprocess
+    from vectorstorekit_b200 import build
+    build.build_library()
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    source, exe = tmp_path / "sizes.cpp", str(tmp_path / "sizes")
+    source.write_text('''
+#include "vectorstorekit_b200/host/vsk.hpp"
+template <typename E, typename F> int refused(F f) { try { f(); } catch (const E&) { return 0; } return 1; }
+int main() {
+  vsk::Int4Quantizer symmetric(nullptr, 32), other(nullptr, 32, false);
+  vsk::Int4Quantizer::Rows r;
+  r.codes.resize(2 * 20);
+  r.scales.resize(2 * 2);
+  int bad = refused<vsk::DimensionMismatch>([&] { symmetric.dequantizeBatch(r, 3, 40); });   // a row too few
+  bad += refused<vsk::DimensionMismatch>([&] { symmetric.dequantizeBatch(r, 2, 65); });      // too many columns
+  bad += refused<vsk::DimensionMismatch>([&] { other.dequantizeBatch(r, 2, 40); });          // no middles
+  bad += refused<vsk::EmptyInput>([&] { symmetric.dequantizeBatch(r, 0, 40); });
+  r.middles.resize(2 * 2);
+  return bad + refused<vsk::DimensionMismatch>([&] { symmetric.dequantizeBatch(r, 2, 40); });
+}
+''')
+    subprocess.run(["g++", "-std=c++17", "-pthread", "-I", root, str(source), "-o", exe, "-L", os.path.join(root, "vectorstorekit_b200"),
+                    "-lvsk_cuda", "-Wl,-rpath," + os.path.join(root, "vectorstorekit_b200")], check=True)
+    assert subprocess.run([exe]).returncode == 0

@@ -594,18 +594,19 @@ int vector_bytes(const vsk_state& s) {
   return (bits & 15) == 0 ? 16 : (bits & 7) == 0 ? 8 : (bits & 3) == 0 ? 4 : (bits & 1) == 0 ? 2 : 1;
 }
 
+// Blocks of a state that moves vectors of `width` bytes; more than a launch has: -1.
+int64_t blocks_of(const vsk_state& s, int width, int64_t batch) {
+  const int64_t tiles = ceil_div(s.steps * s.step_bytes, 256 * kPlaces * (int64_t)width);
+  if (tiles > 0x7fffffffLL || s.outer > 0x7fffffffLL || batch * s.outer > 0x7fffffffLL / tiles) return -1;
+  return batch * s.outer * tiles;
+}
+int move_width(const vsk_state& s, int beams) {
+  const int w = vector_bytes(s);
+  return w == 16 && s.src == s.dst && beams > 32 ? 8 : w;   // (sixty-four vectors of 16 bytes do not fit the registers)
+}
+
 template <typename V>
-int32_t reorder(Ctx* ctx, StateArgs& a, bool in_place) {
-  int64_t blocks = 0;
-  for (int i = 0; i < a.count; ++i) {
-    StateMove& m = a.move[i];
-    const int64_t tiles = ceil_div(m.inner, 256 * kPlaces * (int64_t)sizeof(V));
-    if (tiles > 0x7fffffffLL || m.outer > 0x7fffffffLL || a.batch * m.outer > 0x7fffffffLL / tiles || blocks + a.batch * m.outer * tiles > 0x7fffffffLL)
-      return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "the states are too large for one call");
-    m.first_block = (unsigned)blocks;
-    m.tiles = (unsigned)tiles;
-    blocks += a.batch * m.outer * tiles;
-  }
+int32_t reorder(Ctx* ctx, StateArgs& a, bool in_place, int64_t blocks) {
   if (!in_place || a.beams <= 8) reorder_kernel<V, 8><<<(unsigned)blocks, 256, 0, ctx->stream>>>(a);
   else if (a.beams <= 16) reorder_kernel<V, 16><<<(unsigned)blocks, 256, 0, ctx->stream>>>(a);
   else if (a.beams <= 32) reorder_kernel<V, 32><<<(unsigned)blocks, 256, 0, ctx->stream>>>(a);
@@ -645,6 +646,9 @@ int32_t vsk_beam_select_dev(vsk_ctx* c, const void* logits, int32_t dtype, int64
   if (dtype != VSK_DTYPE_F32 && dtype != VSK_DTYPE_F16 && dtype != VSK_DTYPE_BF16)
     return fail(ctx, VSK_ERR_UNSUPPORTED_OPERATION, "element type %d is not supported", dtype);
   if (reinterpret_cast<uintptr_t>(logits) & (dtype == VSK_DTYPE_F32 ? 3 : 1)) return fail(ctx, VSK_ERR_INVALID_INPUT, "logits are not aligned to their element");
+  if (((reinterpret_cast<uintptr_t>(scores) | reinterpret_cast<uintptr_t>(out_scores)) & 3) ||
+      ((reinterpret_cast<uintptr_t>(out_beams) | reinterpret_cast<uintptr_t>(out_tokens)) & 7))
+    return fail(ctx, VSK_ERR_INVALID_INPUT, "scores, beams or tokens are not aligned to their element");
   drain_stale_error("vsk_beam_select_dev");
   BeamArgs a{};
   a.logits = logits;
@@ -676,6 +680,8 @@ int32_t vsk_reorder_states_dev(vsk_ctx* c, const vsk_state* states, int32_t coun
   if (beams > kMaxBeams) return fail(ctx, VSK_ERR_INVALID_INPUT, "at most %d beams", kMaxBeams);
   if (batch > 0x7fffffffLL) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "batch must be below 2^31");
   if (!states || !parents) return fail(ctx, VSK_ERR_INVALID_INPUT, "null pointer");
+  if ((reinterpret_cast<uintptr_t>(parents) | reinterpret_cast<uintptr_t>(lengths)) & 7)
+    return fail(ctx, VSK_ERR_INVALID_INPUT, "parents or lengths are not aligned to their element");
   for (int32_t i = 0; i < count; ++i) {
     const vsk_state& s = states[i];
     if (!s.src || !s.dst) return fail(ctx, VSK_ERR_INVALID_INPUT, "state %d: null pointer", i);
@@ -687,6 +693,14 @@ int32_t vsk_reorder_states_dev(vsk_ctx* c, const vsk_state* states, int32_t coun
       return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "state %d: rows overlap", i);
     if (s.src == s.dst && (s.src_row_stride != s.dst_row_stride || (s.outer > 1 && s.src_outer_stride != s.dst_outer_stride)))
       return fail(ctx, VSK_ERR_INVALID_INPUT, "state %d: in place, but with other strides", i);
+    if (blocks_of(s, move_width(s, beams), batch) < 0) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "state %d is too large", i);
+    const double last = (double)(batch * beams - 1) * s.dst_row_stride + (double)(s.outer - 1) * (s.outer > 1 ? s.dst_outer_stride : 0) + inner;
+    auto inside = [&](const int64_t* p, int64_t numbers) {
+      const double from = (double)((intptr_t)p - (intptr_t)s.dst);
+      return p && from < last && from + 8. * numbers > 0.;
+    };
+    if (inside(parents, batch * beams) || inside(lengths, batch))
+      return fail(ctx, VSK_ERR_INVALID_INPUT, "parents or lengths lie in state %d, which moves", i);
     for (int32_t j = 0; j < i; ++j)
       if (states[j].dst == s.dst || states[j].src == s.dst || s.src == states[j].dst)
         return fail(ctx, VSK_ERR_INVALID_INPUT, "states %d and %d are the same memory", j, i);
@@ -704,31 +718,38 @@ int32_t vsk_reorder_states_dev(vsk_ctx* c, const vsk_state* states, int32_t coun
       a.parents = parents;
       a.lengths = lengths;
       a.bad = (int*)ctx->host_flags[0].p;
-      for (int32_t i = 0; i <= count; ++i) {
-        if (i < count) {
-          const vsk_state& s = states[i];
-          int w = vector_bytes(s);
-          if (w == 16 && in_place && beams > 32) w = 8;   // (sixty-four vectors of 16 bytes do not fit the registers)
-          if (w != width || (s.src == s.dst) != (in_place == 1)) continue;
-          StateMove& m = a.move[a.count++];
-          m.src = (const uint8_t*)s.src;
-          m.dst = (uint8_t*)s.dst;
-          m.src_row = s.src_row_stride;
-          m.dst_row = s.dst_row_stride;
-          m.src_outer = s.src_outer_stride;
-          m.dst_outer = s.dst_outer_stride;
-          m.outer = s.outer;
-          m.inner = s.steps * s.step_bytes;
-          m.step = s.timed ? s.step_bytes : 0;
-        }
-        if (a.count == 0 || (i < count && a.count < kStatesPerLaunch)) continue;
-        VSK_TRY(width == 16  ? reorder<uint4>(ctx, a, in_place)
-                : width == 8 ? reorder<uint2>(ctx, a, in_place)
-                : width == 4 ? reorder<uint32_t>(ctx, a, in_place)
-                : width == 2 ? reorder<uint16_t>(ctx, a, in_place)
-                             : reorder<uint8_t>(ctx, a, in_place));
+      int64_t blocks = 0;
+      auto launch = [&]() -> int32_t {
+        if (a.count == 0) return VSK_OK;
+        VSK_TRY(width == 16  ? reorder<uint4>(ctx, a, in_place, blocks)
+                : width == 8 ? reorder<uint2>(ctx, a, in_place, blocks)
+                : width == 4 ? reorder<uint32_t>(ctx, a, in_place, blocks)
+                : width == 2 ? reorder<uint16_t>(ctx, a, in_place, blocks)
+                             : reorder<uint8_t>(ctx, a, in_place, blocks));
         a.count = 0;
+        blocks = 0;
+        return VSK_OK;
+      };
+      for (int32_t i = 0; i < count; ++i) {
+        const vsk_state& s = states[i];
+        if (move_width(s, beams) != width || (s.src == s.dst) != (in_place == 1)) continue;
+        const int64_t more = blocks_of(s, width, batch);
+        if (a.count == kStatesPerLaunch || blocks + more > 0x7fffffffLL) VSK_TRY(launch());
+        StateMove& m = a.move[a.count++];
+        m.src = (const uint8_t*)s.src;
+        m.dst = (uint8_t*)s.dst;
+        m.src_row = s.src_row_stride;
+        m.dst_row = s.dst_row_stride;
+        m.src_outer = s.src_outer_stride;
+        m.dst_outer = s.dst_outer_stride;
+        m.outer = s.outer;
+        m.inner = s.steps * s.step_bytes;
+        m.step = s.timed ? s.step_bytes : 0;
+        m.first_block = (unsigned)blocks;
+        m.tiles = (unsigned)(more / (batch * s.outer));
+        blocks += more;
       }
+      VSK_TRY(launch());
     }
   tl_mark(ctx, "reorder_states");
   VSK_CUDA(ctx, cudaStreamSynchronize(ctx->stream));

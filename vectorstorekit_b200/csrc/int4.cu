@@ -390,6 +390,7 @@ int32_t vsk_q4_decode_dev(vsk_ctx* c, const vsk_q4_rows* rows, float* out) {
   VSK_TRY(check_ctx(c, &ctx));
   VSK_TRY(check_rows(ctx, rows));
   if (!out) return fail(ctx, VSK_ERR_INVALID_INPUT, "null pointer");
+  if (reinterpret_cast<uintptr_t>(out) & 3) return fail(ctx, VSK_ERR_INVALID_INPUT, "a pointer is not aligned to its element");
   drain_stale_error("vsk_q4_decode_dev");
   VSK_TRY(decode(ctx, rows, out));
   tl_mark(ctx, "q4_decode");

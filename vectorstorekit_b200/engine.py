@@ -13,6 +13,8 @@ Names, argument meaning and error behaviour follow the reference's Swift types f
   batch search (``API/VectorStore.swift:271-318``, ``LLM/LLMVectorStore.swift:83-114``)
 * ``IVFIndex``                    — ``Indexes/IVFIndex.swift`` train / insert / search
 * ``ScalarQuantizer``             — ``Quantization/ScalarQuantizer.swift`` (int8)
+* ``CUDAAccelerationEngine.selectBeams`` / ``reorderStates`` — no counterpart: a beam search's step over several rows of scores
+  (rows in four bits, whose products give such scores: ``int4.py``)
 
 Arrays may be numpy arrays (host memory: copied in and out by the library) or torch CUDA tensors
 (device memory of the engine's GPU: used in place, results returned as CUDA tensors).
@@ -562,8 +564,9 @@ class CUDAAccelerationEngine:
 
         ``states``: CUDA tensors ``[batch * beams, ...]`` of any element type (key-value caches, token histories).  ``out=None`` moves
         them in place, in any permutation; otherwise into the tensors of ``out`` (same shapes and types, other memory).  ``parents
-        [batch][beams]`` int64; a parent of -1 leaves its row as it is.  ``lengths [batch]`` int64 with ``time_axis`` (one number, or one
-        per state; None for a state without time): only the first ``lengths[b]`` places of that axis move, what lies behind stays.
+        [batch][beams]`` int64, not in a moved state's memory; a parent of -1 leaves its row as it is.  ``lengths [batch]`` int64 with
+        ``time_axis`` (one number, or one per state; None for a state without time): only the first ``lengths[b]`` places of that axis
+        move, what lies behind stays.
         At most 64 beams.  Returns ``out``, or ``states``."""
         states = list(states)
         if not states:

@@ -362,6 +362,11 @@ class Int4Quantizer {
     return r;
   }
   std::vector<float> dequantizeBatch(const Rows& r, int64_t n, int32_t dim) const {
+    if (n <= 0) throw EmptyInput(VSK_ERR_EMPTY_INPUT, "no rows");
+    if (dim <= 0 || group_ <= 0) throw DimensionMismatch(VSK_ERR_DIMENSION_MISMATCH, "dimension and group size must be positive");
+    const size_t scales = (size_t)n * (((size_t)dim + group_ - 1) / group_);
+    if (r.codes.size() != (size_t)n * (((size_t)dim + 1) / 2) || r.scales.size() != scales || r.middles.size() != (symmetric_ ? 0 : scales))
+      throw DimensionMismatch(VSK_ERR_DIMENSION_MISMATCH, "codes, scales or middles do not have the size of these rows");
     std::vector<float> out((size_t)std::max<int64_t>(n, 0) * (size_t)std::max(dim, 0));
     const vsk_q4_rows d = descriptor(r.codes.data(), r.scales.data(), symmetric_ ? nullptr : r.middles.data(), n, dim);
     check(vsk_q4_decode(dev_->ctx(), &d, out.data()), dev_->ctx());
