@@ -449,6 +449,7 @@ int32_t vsk_q4_product_dev(vsk_ctx* c, const vsk_q4_rows* rows, const void* x, i
   // 200 000 x 2 048, groups of 128 / of 32 with middles: four fp16 vectors take 74 / 123 us in whole numbers and 91 / 143 in 16 bits, six
   // 99 / 175 and 91 / 143 (they no longer fit two tiles of digits).  fp32 vectors have no 16-bit form.
   if (x_dtype == VSK_DTYPE_F32 || nq <= 4) VSK_TRY(q4_product_digits(ctx, *rows, x, x_dtype, nq, x_stride, y, y_dtype, y_stride));
+  else if (q4_fits_tensor(ctx, *rows, nq)) return q4_product_tensor(ctx, *rows, x, x_dtype, nq, x_stride, y, y_dtype, y_stride);
   else VSK_TRY(q4_product(ctx, *rows, x, x_dtype, nq, x_stride, y, y_dtype, y_stride));
   tl_mark(ctx, "q4_product");
   VSK_CUDA(ctx, cudaStreamSynchronize(ctx->stream));

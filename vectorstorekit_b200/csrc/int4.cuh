@@ -1,6 +1,10 @@
-// Products with rows in four bits: what int4.cu (checks, entry points) asks of int4_product.cu.
+// Products with rows in four bits: what int4.cu (checks, entry points) asks of the other files.
 #pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -13,6 +17,47 @@ int32_t q4_product(Ctx* ctx, const vsk_q4_rows& rows, const void* x, int32_t x_d
 // The same in whole numbers, for a few vectors (int4_digits.cu).
 int32_t q4_product_digits(Ctx* ctx, const vsk_q4_rows& rows, const void* x, int32_t x_dtype, int64_t nq, int64_t x_stride, void* y,
                           int32_t y_dtype, int64_t y_stride);
+
+// The same on the tensor cores' block form, for rows without middles, at 16-byte places, that fill the machine (int4_tensor.cu).
+bool q4_fits_tensor(Ctx* ctx, const vsk_q4_rows& rows, int64_t nq);
+int32_t q4_product_tensor(Ctx* ctx, const vsk_q4_rows& rows, const void* x, int32_t x_dtype, int64_t nq, int64_t x_stride, void* y,
+                          int32_t y_dtype, int64_t y_stride);
+
+__device__ __forceinline__ void wait_for_launches_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_the_next_launch_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {   // (w & mask) | bits, in one instruction
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+  return r;
+}
+
+// Eight codes to four pairs (code j, code j + 4) of the numbers code - 8, exactly: the code under the exponent of 1024 (fp16) or 128 (bf16)
+// is that power plus the code, and the difference needs no rounding.
+template <typename T>
+__device__ __forceinline__ void unpack(uint32_t w, uint32_t (&p)[4]) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 base = __half2half2(__ushort_as_half(0x6408)), scale = __half2half2(__ushort_as_half(0x2c00)),   // 1032, 1/16
+                  high = __half2half2(__ushort_as_half(0xd480));                                                    // -72
+    const uint32_t v = w >> 8;
+    uint32_t q[4] = {and_or(w, 0x000f000fu, 0x64006400u), and_or(w, 0x00f000f0u, 0x64006400u), and_or(v, 0x000f000fu, 0x64006400u),
+                     and_or(v, 0x00f000f0u, 0x64006400u)};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      __half2 h = *reinterpret_cast<__half2*>(&q[j]);
+      h = (j & 1) ? __hfma2(h, scale, high) : __hsub2(h, base);   // (1024 + 16 c) / 16 - 72 = c - 8
+      p[j] = *reinterpret_cast<uint32_t*>(&h);
+    }
+  } else {
+    const __nv_bfloat162 base = __bfloat162bfloat162(__ushort_as_bfloat16(0x4308));   // 136
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t q = and_or(w >> (4 * j), 0x000f000fu, 0x43004300u);
+      __nv_bfloat162 h = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&q), base);
+      p[j] = *reinterpret_cast<uint32_t*>(&h);
+    }
+  }
+}
 
 // Warps of a block that share a tile's columns: what leaves the busiest warp the fewest steps (a tile's end counts as one), tiles being dealt
 // out to `slots` warps.  39 865 x 7 680, one fp16 vector: one warp each 60 steps for half the warps, eight 5 x 8.

@@ -1,13 +1,13 @@
 // Products of tens of vectors with rows held in four bits (int4.cu has the format, int4_digits.cu the form for a few vectors).
 //
 // Here x stays in its 16 bits and the codes become exact 16-bit numbers, so that the call is bound by the tensor cores' warp form
-// (m16n8k16, fp32 sums) rather than by three digits' worth of columns: a code under the exponent of 1024 (fp16) or 128 (bf16) is that power
+// (m16n8k16, fp32 sums) rather than by four digits' worth of columns: a code under the exponent of 1024 (fp16) or 128 (bf16) is that power
 // plus the code, and taking the power and 8 away needs no rounding.  A group's sum is taken in fp32 registers, multiplied by the
 // scale there and added to the row's total: codes are never multiplied by a rounded weight.
 //
-// 131 072 x 2 048, groups of 128, 32 bf16 vectors: 104 us, 165 TFLOP/s, where the warp form's rate would allow 31 us and the bytes 24:
-// tensor pipe 33 %, issue slots 32 %, each warp alternating between unpacking and products.  No variant tried brought the two together:
-// four tiles of rows per warp, 2 - 6 stages, two blocks per SM, sixteen warps in step with x in shared memory were all within 7 %.
+// Rows that fill the machine at 16-byte places, without middles, go to int4_tensor.cu.  131 072 x 2 048, groups of 128, 32 bf16 vectors, here: 104 us,
+// where the warp form's rate would allow 31: tensor pipe 33 %, issue slots 32 %, each warp alternating between unpacking and products.  Four tiles
+// of rows per warp, 2 - 6 stages, two blocks per SM, sixteen warps in step with x in shared memory were all within 7 %.
 //
 //   codes   32 rows x 128 columns (2 KB) per step into a ring in shared memory that belongs to ONE warp, by asynchronous 16-byte copies.  A
 //           lane's words of a group lie side by side where the group is that wide, and the pieces of a row are turned so that the rows read
@@ -16,8 +16,6 @@
 //           is launched with it and has its first codes under way before it waits for it
 //   scales  asked for by the row's lane two steps ahead, handed to the fragments' lanes as fp32 numbers in shared memory; middles likewise,
 //           times the vectors' sums over the group
-#include <cuda_bf16.h>
-
 #include <algorithm>
 
 #include "int4.cuh"
@@ -55,8 +53,6 @@ __device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) 
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void wait_for_launches_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void let_the_next_launch_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const float (&c)[4]) {
@@ -68,39 +64,6 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
-  }
-}
-
-__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {   // (w & mask) | bits, in one instruction
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
-  return r;
-}
-
-// Eight codes to four pairs (code j, code j + 4) of the numbers code - 8, exactly: the code under the exponent of 1024 (fp16) or 128 (bf16)
-// is that power plus the code, and the difference needs no rounding.
-template <typename T>
-__device__ __forceinline__ void unpack(uint32_t w, uint32_t (&p)[4]) {
-  if constexpr (std::is_same<T, __half>::value) {
-    const __half2 base = __half2half2(__ushort_as_half(0x6408)), scale = __half2half2(__ushort_as_half(0x2c00)),   // 1032, 1/16
-                  high = __half2half2(__ushort_as_half(0xd480));                                                    // -72
-    const uint32_t v = w >> 8;
-    uint32_t q[4] = {and_or(w, 0x000f000fu, 0x64006400u), and_or(w, 0x00f000f0u, 0x64006400u), and_or(v, 0x000f000fu, 0x64006400u),
-                     and_or(v, 0x00f000f0u, 0x64006400u)};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      __half2 h = *reinterpret_cast<__half2*>(&q[j]);
-      h = (j & 1) ? __hfma2(h, scale, high) : __hsub2(h, base);   // (1024 + 16 c) / 16 - 72 = c - 8
-      p[j] = *reinterpret_cast<uint32_t*>(&h);
-    }
-  } else {
-    const __nv_bfloat162 base = __bfloat162bfloat162(__ushort_as_bfloat16(0x4308));   // 136
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t q = and_or(w >> (4 * j), 0x000f000fu, 0x43004300u);
-      __nv_bfloat162 h = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&q), base);
-      p[j] = *reinterpret_cast<uint32_t*>(&h);
-    }
   }
 }
 

@@ -1,0 +1,387 @@
+// Products of tens of 16-bit vectors with many rows held in four bits, on tcgen05 (int4_product.cu has the warp form and its reasons).
+//
+// A wait that runs out ends the block's part with what it has: the call returns VSK_ERR_TIMEOUT.
+//
+// A block takes 128 rows (the matrix instruction's M) and NV = 16 or 32 vectors (its N).  Per step of 64 columns
+//   codes     32 bytes per row, two lanes a row, asked for two steps ahead; they become exact 16-bit numbers (code - 8) that are written
+//             to shared memory as the instruction wants them: rows of 128 bytes, 16-byte pieces turned by the row (128-byte swizzle).  A word of
+//             eight codes is one piece; its columns come in the order 0 4 1 5 2 6 3 7, which the vectors' tile has too
+//   vectors   NV rows of 128 bytes, brought into that order and turned once by a kernel of its own; a step's tile is copied as it is
+//   products  four instructions of 16 columns, sums of one group of columns per accumulator in tensor memory
+//   scales    a thread owns a row: it reads the group's sums of its row, multiplies by the scale in fp32 and adds to the row's NV totals, while
+//             the next step's products run.  Accumulators, operands and barriers are double
+// Codes are never multiplied by a rounded weight: every product is exact, sums are fp32.
+//
+// 131 072 x 2 048, groups of 128, 32 bf16 vectors: the call takes 97 us, 127 with the warp form.
+#include "int4.cuh"
+#include "tc_ptx.cuh"
+
+namespace vsk {
+namespace {
+using namespace tc;
+
+constexpr int kThreads = 128;
+constexpr int kBlocks = 4;         // per SM: accumulators of 4 x 128 columns are all of the tensor memory
+constexpr int kStepBytes = 128 * 128;
+
+struct TensorArgs {
+  const uint8_t* codes;
+  int64_t code_stride;
+  const __half* scales;
+  int64_t scale_stride;
+  int64_t n;
+  int row_bytes, groups, steps;   // steps of 64 columns
+  int quads;                      // four scales of a row can be read at once
+  const uint4* x;                 // [chunk][step][NV][8 pieces, turned]
+  int64_t nq;
+  void* y;
+  int64_t y_stride;
+  int y_dtype;
+  int* err;                       // pinned: a wait ran out
+};
+
+template <int NV, int GROUP>
+struct Shape {
+  static constexpr int kPer = GROUP == 32 ? 2 : 1;                         // groups that end in a step, at most
+  static constexpr int kColumns = 2 * NV * kPer;                           // of tensor memory: 32, 64 or 128
+  static constexpr int kTile = NV * 128;
+  static constexpr int kShared = 2 * kStepBytes + 2 * kTile + 1024;        // (the swizzle counts from multiples of 1 024)
+  // so much that no fifth block's accumulators would have to wait for tensor memory
+  static constexpr int kAsked = kShared > 47 * 1024 ? kShared : 47 * 1024;
+};
+
+template <int NV>
+__device__ __forceinline__ void load_sums(uint32_t at, float (&v)[NV]) {
+  if constexpr (NV == 32) {
+    tc_ld32(at, v);
+  } else {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+                   "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+                 : "r"(at)
+                 : "memory");
+    tc_ld_wait();
+  }
+}
+
+// False when the limit of looks has run out.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) {
+  for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (i > 64) __nanosleep(64);
+  }
+  return false;
+}
+
+template <typename T, int NV, int GROUP>
+__global__ void __launch_bounds__(kThreads, kBlocks) q4_tensor_kernel(const __grid_constant__ TensorArgs a) {
+  using S = Shape<NV, GROUP>;
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t done[2];
+  __shared__ uint32_t tmem_at;
+  __shared__ int gave_up;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* const rows_at = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+  uint8_t* const x_at = rows_at + 2 * kStepBytes;
+  if (threadIdx.x == 0) {
+    mbar_init(&done[0], 1);
+    mbar_init(&done[1], 1);
+    gave_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_at)), "r"(S::kColumns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_at;
+
+  const int64_t q0 = (int64_t)blockIdx.y * NV;
+  const int nq = (int)min((int64_t)NV, a.nq - q0);
+  const int tiles = (int)((a.n + 127) / 128);
+  const int mine = (int)blockIdx.x < tiles ? (tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+  const int64_t total = (int64_t)mine * a.steps;
+
+  // The codes of two steps: this lane's half of rows lane / 2 and sixteen more of the warp's 32.  Rows behind the last repeat it; bytes behind a
+  // row's end are zeros, whose columns of the vectors are zero.
+  const int half = lane & 1, first = warp * 32 + (lane >> 1);
+  int f_tile = blockIdx.x, f_step = 0;
+  const uint8_t* f_src[2];
+  auto aim = [&]() {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) f_src[j] = a.codes + min((int64_t)f_tile * 128 + first + 16 * j, a.n - 1) * a.code_stride + half * 16;
+  };
+  aim();
+  uint4 held[2][2];
+  auto fetch = [&](uint4 (&to)[2]) {
+    if (f_tile >= tiles) return;
+    const int have = a.row_bytes - f_step * 32 - half * 16;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (have >= 16) {
+        to[j] = *VSK_CHK(reinterpret_cast<const uint4*>(f_src[j]));
+      } else {
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int b = 0; b < 15; ++b)
+          if (b < have) w[b >> 2] |= (uint32_t)*VSK_CHK(f_src[j] + b) << (8 * (b & 3));
+        to[j] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      f_src[j] += 32;
+    }
+    if (++f_step == a.steps) {
+      f_step = 0;
+      f_tile += gridDim.x;
+      aim();
+    }
+  };
+  fetch(held[0]);
+  fetch(held[1]);
+
+  // the scales of this thread's row, four groups at a time, the next four under way
+  int s_tile = blockIdx.x, s_group = 0;
+  auto scales_of_four = [&]() {
+    uint2 v = make_uint2(0, 0);
+    if (s_tile < tiles) {
+      const __half* at = a.scales + min((int64_t)s_tile * 128 + threadIdx.x, a.n - 1) * a.scale_stride + s_group;
+      if (a.quads && s_group + 4 <= a.groups) {
+        v = *VSK_CHK(reinterpret_cast<const uint2*>(at));
+      } else {
+        uint32_t h[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[e] = s_group + e < a.groups ? __half_as_ushort(*VSK_CHK(at + e)) : 0;
+        v = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+      }
+      s_group += 4;
+      if (s_group >= a.groups) {
+        s_group = 0;
+        s_tile += gridDim.x;
+      }
+    }
+    return v;
+  };
+  uint2 scales = make_uint2(0, 0), scales_next = scales_of_four();
+
+  float tot[NV];
+#pragma unroll
+  for (int q = 0; q < NV; ++q) tot[q] = 0.f;
+
+  wait_for_launches_before();   // x
+  const uint4* const x0 = a.x + (int64_t)blockIdx.y * a.steps * (NV * 8) + threadIdx.x;
+  uint4 xs[NV / 16];
+  int x_step = 0;
+  auto fetch_x = [&]() {
+#pragma unroll
+    for (int j = 0; j < NV / 16; ++j) xs[j] = *VSK_CHK(x0 + (int64_t)x_step * (NV * 8) + j * kThreads);
+    x_step = x_step + 1 == a.steps ? 0 : x_step + 1;
+  };
+  fetch_x();
+
+  bool ok = true;
+  int group = 0;              // of the row: the next one whose sums are taken
+  int issued = 0, taken = 0;  // groups so far: their accumulators alternate
+  // The sums of the step before `at` steps: waits for its products, and takes the groups that ended with them.
+  auto finish = [&](int64_t at, bool ends) {
+    if (ok) ok = wait_for(&done[at & 1], (uint32_t)(at >> 1) & 1u);
+    __syncwarp();
+    if (!ends) return;
+    tc_fence_after();
+    const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16) + (taken & 1) * (NV * S::kPer);
+#pragma unroll
+    for (int e = 0; e < S::kPer; ++e) {
+      float v[NV];
+      load_sums<NV>(from + e * NV, v);
+      if ((group & 3) == 0) {
+        scales = scales_next;
+        scales_next = scales_of_four();
+      }
+      const uint32_t pair = (group & 2) ? scales.y : scales.x;
+      const float s = __half2float(__ushort_as_half((unsigned short)((group & 1) ? pair >> 16 : pair)));
+      if (group < a.groups) {
+#pragma unroll
+        for (int q = 0; q < NV; ++q) tot[q] = fmaf(s, v[q], tot[q]);
+        ++group;
+      }
+    }
+    ++taken;
+  };
+  // whether a step is its group's (or groups') last
+  auto ends_group = [&](int step) { return GROUP != 128 || (step & 1) || step == a.steps - 1; };
+
+  constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
+  constexpr uint32_t kInstruction = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(NV >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+  int step = 0;
+  int64_t tile = blockIdx.x;
+  auto body = [&](int64_t at, auto which) {
+    constexpr int B = decltype(which)::value;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = first + 16 * j;
+      const uint32_t w[4] = {held[B][j].x, held[B][j].y, held[B][j].z, held[B][j].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t p[4];
+        unpack<T>(w[i], p);
+        *reinterpret_cast<uint4*>(rows_at + B * kStepBytes + r * 128 + (((half * 4 + i) ^ (r & 7)) * 16)) = make_uint4(p[0], p[1], p[2], p[3]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NV / 16; ++j) *reinterpret_cast<uint4*>(x_at + B * S::kTile + (threadIdx.x + j * kThreads) * 16) = xs[j];
+    fetch(held[B]);
+    fetch_x();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+      tc_fence_after();
+      if (elect_one() && ok) {
+        const uint32_t lo_a = desc_lo(smem_u32(rows_at + B * kStepBytes)), lo_b = desc_lo(smem_u32(x_at + B * S::kTile));
+        const uint32_t to = tmem + (issued & 1) * (NV * S::kPer);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t more = GROUP == 128 ? (uint32_t)(k > 0 || (step & 1)) : GROUP == 64 ? (uint32_t)(k > 0) : (uint32_t)(k & 1);
+          tc_mma(GROUP == 32 ? to + (k >> 1) * NV : to, desc_pack(lo_a + k * 2, kDescHi), desc_pack(lo_b + k * 2, kDescHi), kInstruction, more);
+        }
+        tc_commit(&done[B]);
+      }
+      __syncwarp();
+    }
+    if (step > 0) finish(at - 1, ends_group(step - 1));
+    if (ends_group(step)) ++issued;
+    if (++step < a.steps) return;
+    // the tile's end: the last step's sums, and the results
+    finish(at, true);
+    const int64_t row = tile * 128 + threadIdx.x;
+    if (row < a.n) {
+      auto put = [&](auto* y, auto&& rounded) {
+        auto* p = y + q0 * a.y_stride + row;
+#pragma unroll
+        for (int q = 0; q < NV; ++q) {
+          if (q < nq) *VSK_CHK_W(p) = rounded(tot[q]);
+          p += a.y_stride;
+        }
+      };
+      if (a.y_dtype == VSK_DTYPE_F32) put((float*)a.y, [](float v) { return v; });
+      else if (a.y_dtype == VSK_DTYPE_F16) put((__half*)a.y, [](float v) { return __float2half_rn(v); });
+      else put((__nv_bfloat16*)a.y, [](float v) { return __float2bfloat16_rn(v); });
+    }
+#pragma unroll
+    for (int q = 0; q < NV; ++q) tot[q] = 0.f;
+    // (four scales are taken when a row's groups begin anew)
+    group = 0;
+    step = 0;
+    tile += gridDim.x;
+  };
+#pragma unroll 1
+  for (int64_t at = 0; at < total; at += 2) {
+    body(at, std::integral_constant<int, 0>());
+    if (at + 1 < total) body(at + 1, std::integral_constant<int, 1>());
+  }
+  if (!ok) {
+    gave_up = 1;
+    wait_for(&done[(total - 1) & 1], (uint32_t)((total - 1) >> 1) & 1u);   // what is still under way, with the same limit
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && gave_up) *reinterpret_cast<volatile int*>(a.err) = 1;
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kColumns) : "memory");
+  }
+}
+
+// x as the steps' tiles, zeros behind dim and behind the last vector: a thread per eight columns of one vector.
+template <typename T>
+__global__ void __launch_bounds__(128) q4_to_tiles_kernel(const T* __restrict__ x, int64_t x_stride, int64_t nq, int64_t q_first, int dim, int steps,
+                                                          int nv, uint4* __restrict__ out) {
+  let_the_next_launch_begin();
+  const int64_t q = q_first + blockIdx.y;
+  const int p = blockIdx.x * 128 + threadIdx.x, col = p * 8;
+  if (p >= steps * 8) return;
+  __align__(16) T v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = q < nq && col + j < dim ? *VSK_CHK(x + q * x_stride + col + j) : T(0.f);
+  __align__(16) T w[8] = {v[0], v[4], v[1], v[5], v[2], v[6], v[3], v[7]};   // as the codes of a word are taken apart
+  const int c = (int)(q % nv);
+  *VSK_CHK_W(out + ((q / nv * steps + (p >> 3)) * nv + c) * 8 + ((p & 7) ^ (c & 7))) = *reinterpret_cast<const uint4*>(w);
+}
+
+template <typename T, int NV, int GROUP>
+int32_t launch(Ctx* ctx, const TensorArgs& a) {
+  using S = Shape<NV, GROUP>;
+  auto kernel = q4_tensor_kernel<T, NV, GROUP>;
+  VSK_CUDA(ctx, opt_in_shared(ctx, kernel, S::kAsked));
+  const int64_t chunks = ceil_div(a.nq, NV), tiles = ceil_div(a.n, 128);
+  const int64_t blocks = std::min(tiles, std::max<int64_t>(1, (int64_t)ctx->prop.multiProcessorCount * kBlocks / chunks));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)blocks, (unsigned)chunks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kAsked;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  VSK_CUDA(ctx, cudaLaunchKernelEx(&cfg, kernel, a));
+  ctx->stats.kernel_launches++;
+  return VSK_OK;
+}
+
+template <typename T>
+int32_t prepare_and_launch(Ctx* ctx, const TensorArgs& a, const T* x, int64_t x_stride, int dim, int group, int nv) {
+  const int64_t vectors = ceil_div(a.nq, nv) * nv;
+  for (int64_t q = 0; q < vectors; q += 65535) {
+    q4_to_tiles_kernel<T><<<dim3((unsigned)ceil_div(a.steps * 8, 128), (unsigned)std::min<int64_t>(65535, vectors - q)), 128, 0, ctx->stream>>>(
+        x, x_stride, a.nq, q, dim, a.steps, nv, (uint4*)a.x);
+    ctx->stats.kernel_launches++;
+    VSK_CUDA(ctx, cudaGetLastError());
+  }
+  if (nv == 16) return group == 32 ? launch<T, 16, 32>(ctx, a) : group == 64 ? launch<T, 16, 64>(ctx, a) : launch<T, 16, 128>(ctx, a);
+  return group == 32 ? launch<T, 32, 32>(ctx, a) : group == 64 ? launch<T, 32, 64>(ctx, a) : launch<T, 32, 128>(ctx, a);
+}
+
+}  // namespace
+
+// A tile of 128 rows for every SM: with fewer the warp form, which shares a tile's columns among warps, fills the machine better.
+bool q4_fits_tensor(Ctx* ctx, const vsk_q4_rows& rows, int64_t nq) {
+  const uintptr_t code_bits = reinterpret_cast<uintptr_t>(rows.codes) | (uintptr_t)rows.code_stride;
+  return !rows.middles && (code_bits & 15) == 0 && rows.n >= 128 * (int64_t)ctx->prop.multiProcessorCount && ceil_div(rows.n, 128) < (1 << 30) &&
+         nq <= 16 * 65535;
+}
+
+int32_t q4_product_tensor(Ctx* ctx, const vsk_q4_rows& rows, const void* x, int32_t x_dtype, int64_t nq, int64_t x_stride, void* y,
+                          int32_t y_dtype, int64_t y_stride) {
+  TensorArgs a{};
+  a.codes = rows.codes;
+  a.code_stride = rows.code_stride;
+  a.scales = (const __half*)rows.scales;
+  a.scale_stride = rows.scale_stride;
+  a.n = rows.n;
+  a.row_bytes = (rows.dim + 1) / 2;
+  a.groups = (int)ceil_div(rows.dim, rows.group);
+  a.steps = (int)ceil_div(rows.dim, 64);
+  a.quads = ((reinterpret_cast<uintptr_t>(rows.scales) | (uintptr_t)(2 * rows.scale_stride)) & 7) == 0;
+  a.nq = nq;
+  a.y = y;
+  a.y_stride = y_stride;
+  a.y_dtype = y_dtype;
+  const int nv = nq <= 16 ? 16 : 32;
+  void* p;
+  VSK_TRY(scratch(ctx, SLOT_Q16, (size_t)ceil_div(nq, nv) * nv * a.steps * 128, &p));
+  a.x = (const uint4*)p;
+  VSK_TRY(pinned_reserve(ctx, &ctx->host_flags[0], sizeof(int)));
+  volatile int* gave_up = (volatile int*)ctx->host_flags[0].p;
+  *gave_up = 0;
+  a.err = (int*)ctx->host_flags[0].p;
+  VSK_TRY(x_dtype == VSK_DTYPE_F16 ? prepare_and_launch(ctx, a, (const __half*)x, x_stride, rows.dim, rows.group, nv)
+                                   : prepare_and_launch(ctx, a, (const __nv_bfloat16*)x, x_stride, rows.dim, rows.group, nv));
+  tl_mark(ctx, "q4_product");
+  VSK_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+  if (*gave_up) return fail(ctx, VSK_ERR_TIMEOUT, "products with rows in four bits: a bounded wait ran out");
+  return VSK_OK;
+}
+
+}  // namespace vsk
