@@ -3,10 +3,11 @@
 // A wait that runs out ends the block's part with what it has: the call returns VSK_ERR_TIMEOUT.
 //
 // A block takes 128 rows (the matrix instruction's M) and NV = 16 or 32 vectors (its N).  Per step of 64 columns
-//   codes     32 bytes per row, two lanes a row, asked for two steps ahead; they become exact 16-bit numbers (code - 8) that are written
-//             to shared memory as the instruction wants them: rows of 128 bytes, 16-byte pieces turned by the row (128-byte swizzle).  A word of
-//             eight codes is one piece; its columns come in the order 0 4 1 5 2 6 3 7, which the vectors' tile has too
-//   vectors   NV rows of 128 bytes, brought into that order and turned once by a kernel of its own; a step's tile is copied as it is
+//   codes     32 bytes per row, asked for two steps ahead by two lanes that then exchange halves, so that a thread owns a row; they become exact
+//             16-bit numbers (code - 8) in tensor memory, the instruction's left side.  A word of eight codes is four columns there, in the
+//             order 0 4 1 5 2 6 3 7, which the vectors' tile has too
+//   vectors   NV rows of 128 bytes, brought into that order and turned by the row (128-byte swizzle) once by a kernel of its own; a step's tile
+//             is copied to shared memory as it is
 //   products  four instructions of 16 columns, sums of one group of columns per accumulator in tensor memory
 //   scales    a thread owns a row: it reads the group's sums of its row, multiplies by the scale in fp32 and adds to the row's NV totals, while
 //             the next step's products run.  Accumulators, operands and barriers are double
@@ -21,8 +22,8 @@ namespace {
 using namespace tc;
 
 constexpr int kThreads = 128;
-constexpr int kBlocks = 4;         // per SM: accumulators of 4 x 128 columns are all of the tensor memory
-constexpr int kStepBytes = 128 * 128;
+constexpr int kLeft = 32;           // columns of tensor memory that a step's codes take: 64 numbers of 16 bits
+
 
 struct TensorArgs {
   const uint8_t* codes;
@@ -43,11 +44,12 @@ struct TensorArgs {
 template <int NV, int GROUP>
 struct Shape {
   static constexpr int kPer = GROUP == 32 ? 2 : 1;                         // groups that end in a step, at most
-  static constexpr int kColumns = 2 * NV * kPer;                           // of tensor memory: 32, 64 or 128
+  static constexpr int kSums = 2 * NV * kPer;                              // columns of tensor memory: 32, 64 or 128, behind two steps' codes
+  static constexpr int kColumns = 2 * kLeft + kSums <= 128 ? 128 : 256;
+  static constexpr int kBlocks = 512 / kColumns;                           // per SM
   static constexpr int kTile = NV * 128;
-  static constexpr int kShared = 2 * kStepBytes + 2 * kTile + 1024;        // (the swizzle counts from multiples of 1 024)
-  // so much that no fifth block's accumulators would have to wait for tensor memory
-  static constexpr int kAsked = kShared > 47 * 1024 ? kShared : 47 * 1024;
+  // so much that no further block would have to wait for tensor memory
+  static constexpr int kAsked = kBlocks == 4 ? 47 * 1024 : 78 * 1024;
 };
 
 template <int NV>
@@ -64,6 +66,28 @@ __device__ __forceinline__ void load_sums(uint32_t at, float (&v)[NV]) {
   }
 }
 
+// 32 columns of this thread's lane; done behind a tcgen05.wait::st.
+__device__ __forceinline__ void store_codes(uint32_t at, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+// Sums (+)= left (tensor memory, 128 rows of 16 numbers in eight columns) x right (shared memory): one instruction.
+__device__ __forceinline__ void multiply(uint32_t sums, uint32_t left, uint64_t right, uint32_t instruction, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(sums),
+      "r"(left), "l"(right), "r"(instruction), "r"(accumulate)
+      : "memory");
+}
+
 // False when the limit of looks has run out.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) {
   for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
@@ -74,15 +98,14 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) {
 }
 
 template <typename T, int NV, int GROUP>
-__global__ void __launch_bounds__(kThreads, kBlocks) q4_tensor_kernel(const __grid_constant__ TensorArgs a) {
+__global__ void __launch_bounds__(kThreads, (Shape<NV, GROUP>::kBlocks)) q4_tensor_kernel(const __grid_constant__ TensorArgs a) {
   using S = Shape<NV, GROUP>;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t done[2];
   __shared__ uint32_t tmem_at;
   __shared__ int gave_up;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint8_t* const rows_at = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
-  uint8_t* const x_at = rows_at + 2 * kStepBytes;
+  uint8_t* const x_at = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);   // (the swizzle counts from multiples of 1 024)
   if (threadIdx.x == 0) {
     mbar_init(&done[0], 1);
     mbar_init(&done[1], 1);
@@ -96,7 +119,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) q4_tensor_kernel(const __gr
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_at;
+  const uint32_t tmem = tmem_at, own_lanes = (uint32_t)(warp * 32) << 16, sums_at = tmem + 2 * kLeft;
 
   const int64_t q0 = (int64_t)blockIdx.y * NV;
   const int nq = (int)min((int64_t)NV, a.nq - q0);
@@ -104,14 +127,14 @@ __global__ void __launch_bounds__(kThreads, kBlocks) q4_tensor_kernel(const __gr
   const int mine = (int)blockIdx.x < tiles ? (tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
   const int64_t total = (int64_t)mine * a.steps;
 
-  // The codes of two steps: this lane's half of rows lane / 2 and sixteen more of the warp's 32.  Rows behind the last repeat it; bytes behind a
-  // row's end are zeros, whose columns of the vectors are zero.
-  const int half = lane & 1, first = warp * 32 + (lane >> 1);
+  // The codes of two steps: this lane's half of its own row and of its neighbour's.  Rows behind the last repeat it; bytes behind a row's end are
+  // zeros, whose columns of the vectors are zero.
+  const int half = lane & 1, first = threadIdx.x & ~1;
   int f_tile = blockIdx.x, f_step = 0;
   const uint8_t* f_src[2];
   auto aim = [&]() {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) f_src[j] = a.codes + min((int64_t)f_tile * 128 + first + 16 * j, a.n - 1) * a.code_stride + half * 16;
+    for (int j = 0; j < 2; ++j) f_src[j] = a.codes + min((int64_t)f_tile * 128 + first + j, a.n - 1) * a.code_stride + half * 16;
   };
   aim();
   uint4 held[2][2];
@@ -186,9 +209,9 @@ __global__ void __launch_bounds__(kThreads, kBlocks) q4_tensor_kernel(const __gr
   auto finish = [&](int64_t at, bool ends) {
     if (ok) ok = wait_for(&done[at & 1], (uint32_t)(at >> 1) & 1u);
     __syncwarp();
-    if (!ends) return;
     tc_fence_after();
-    const uint32_t from = tmem + ((uint32_t)(warp * 32) << 16) + (taken & 1) * (NV * S::kPer);
+    if (!ends) return;
+    const uint32_t from = sums_at + own_lanes + (taken & 1) * (NV * S::kPer);
 #pragma unroll
     for (int e = 0; e < S::kPer; ++e) {
       float v[NV];
@@ -201,7 +224,11 @@ __global__ void __launch_bounds__(kThreads, kBlocks) q4_tensor_kernel(const __gr
       const float s = __half2float(__ushort_as_half((unsigned short)((group & 1) ? pair >> 16 : pair)));
       if (group < a.groups) {
 #pragma unroll
-        for (int q = 0; q < NV; ++q) tot[q] = fmaf(s, v[q], tot[q]);
+        for (int q = 0; q < NV; q += 2) {
+          const float2 r = __ffma2_rn(make_float2(s, s), make_float2(v[q], v[q + 1]), make_float2(tot[q], tot[q + 1]));
+          tot[q] = r.x;
+          tot[q + 1] = r.y;
+        }
         ++group;
       }
     }
@@ -216,33 +243,40 @@ __global__ void __launch_bounds__(kThreads, kBlocks) q4_tensor_kernel(const __gr
   int64_t tile = blockIdx.x;
   auto body = [&](int64_t at, auto which) {
     constexpr int B = decltype(which)::value;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int r = first + 16 * j;
-      const uint32_t w[4] = {held[B][j].x, held[B][j].y, held[B][j].z, held[B][j].w};
+    {
+      const uint4 mine_of = half ? held[B][1] : held[B][0], other = half ? held[B][0] : held[B][1];
+      const uint32_t kept[4] = {mine_of.x, mine_of.y, mine_of.z, mine_of.w}, given[4] = {other.x, other.y, other.z, other.w};
+      uint32_t p[32];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        uint32_t p[4];
-        unpack<T>(w[i], p);
-        *reinterpret_cast<uint4*>(rows_at + B * kStepBytes + r * 128 + (((half * 4 + i) ^ (r & 7)) * 16)) = make_uint4(p[0], p[1], p[2], p[3]);
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, given[i], 1);
+        uint32_t lo[4], hi[4];
+        unpack<T>(half ? got : kept[i], lo);
+        unpack<T>(half ? kept[i] : got, hi);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[i * 4 + e] = lo[e];
+          p[16 + i * 4 + e] = hi[e];
+        }
       }
+      store_codes(tmem + own_lanes + B * kLeft, p);
     }
 #pragma unroll
     for (int j = 0; j < NV / 16; ++j) *reinterpret_cast<uint4*>(x_at + B * S::kTile + (threadIdx.x + j * kThreads) * 16) = xs[j];
     fetch(held[B]);
     fetch_x();
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
     tc_fence_before();
     __syncthreads();
     if (warp == 0) {
       tc_fence_after();
       if (elect_one() && ok) {
-        const uint32_t lo_a = desc_lo(smem_u32(rows_at + B * kStepBytes)), lo_b = desc_lo(smem_u32(x_at + B * S::kTile));
-        const uint32_t to = tmem + (issued & 1) * (NV * S::kPer);
+        const uint32_t lo_b = desc_lo(smem_u32(x_at + B * S::kTile)), to = sums_at + (issued & 1) * (NV * S::kPer);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const uint32_t more = GROUP == 128 ? (uint32_t)(k > 0 || (step & 1)) : GROUP == 64 ? (uint32_t)(k > 0) : (uint32_t)(k & 1);
-          tc_mma(GROUP == 32 ? to + (k >> 1) * NV : to, desc_pack(lo_a + k * 2, kDescHi), desc_pack(lo_b + k * 2, kDescHi), kInstruction, more);
+          multiply(GROUP == 32 ? to + (k >> 1) * NV : to, tmem + B * kLeft + k * 8, desc_pack(lo_b + k * 2, kDescHi), kInstruction, more);
         }
         tc_commit(&done[B]);
       }
@@ -314,7 +348,7 @@ int32_t launch(Ctx* ctx, const TensorArgs& a) {
   auto kernel = q4_tensor_kernel<T, NV, GROUP>;
   VSK_CUDA(ctx, opt_in_shared(ctx, kernel, S::kAsked));
   const int64_t chunks = ceil_div(a.nq, NV), tiles = ceil_div(a.n, 128);
-  const int64_t blocks = std::min(tiles, std::max<int64_t>(1, (int64_t)ctx->prop.multiProcessorCount * kBlocks / chunks));
+  const int64_t blocks = std::min(tiles, std::max<int64_t>(1, (int64_t)ctx->prop.multiProcessorCount * S::kBlocks / chunks));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)blocks, (unsigned)chunks);
   cfg.blockDim = dim3(kThreads);
