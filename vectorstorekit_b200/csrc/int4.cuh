@@ -23,6 +23,14 @@ bool q4_fits_tensor(Ctx* ctx, const vsk_q4_rows& rows, int64_t nq);
 int32_t q4_product_tensor(Ctx* ctx, const vsk_q4_rows& rows, const void* x, int32_t x_dtype, int64_t nq, int64_t x_stride, void* y,
                           int32_t y_dtype, int64_t y_stride);
 
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {   // bytes behind `bytes` become zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void wait_for_launches_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_the_next_launch_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -3,17 +3,17 @@
 // A wait that runs out ends the block's part with what it has: the call returns VSK_ERR_TIMEOUT.
 //
 // A block takes 128 rows (the matrix instruction's M) and NV = 16 or 32 vectors (its N).  Per step of 64 columns
-//   codes     32 bytes per row, asked for two steps ahead by two lanes that then exchange halves, so that a thread owns a row; they become exact
+//   codes     32 bytes per row, copied to a warp's part of a ring by two lanes a row, four steps ahead; a thread takes its row's, which become exact
 //             16-bit numbers (code - 8) in tensor memory, the instruction's left side.  A word of eight codes is four columns there, in the
 //             order 0 4 1 5 2 6 3 7, which the vectors' tile has too
 //   vectors   NV rows of 128 bytes, brought into that order and turned by the row (128-byte swizzle) once by a kernel of its own; a step's tile
-//             is copied to shared memory as it is
+//             is copied to the ring as it is
 //   products  four instructions of 16 columns, sums of one group of columns per accumulator in tensor memory
 //   scales    a thread owns a row: it reads the group's sums of its row, multiplies by the scale in fp32 and adds to the row's NV totals, while
 //             the next step's products run.  Accumulators, operands and barriers are double
 // Codes are never multiplied by a rounded weight: every product is exact, sums are fp32.
 //
-// 131 072 x 2 048, groups of 128, 32 bf16 vectors: the call takes 97 us, 127 with the warp form.
+// 131 072 x 2 048, groups of 128, 32 bf16 vectors: the call takes 84 us, 127 with the warp form.
 #include "int4.cuh"
 #include "tc_ptx.cuh"
 
@@ -22,6 +22,8 @@ namespace {
 using namespace tc;
 
 constexpr int kThreads = 128;
+constexpr int kStages = 5;
+constexpr int kCodes = 4096 + 16;   // of a stage: even rows, 16 bytes, odd rows (so that the rows of a read lie in different banks)
 constexpr int kLeft = 32;           // columns of tensor memory that a step's codes take: 64 numbers of 16 bits
 
 
@@ -50,6 +52,7 @@ struct Shape {
   static constexpr int kTile = NV * 128;
   // so much that no further block would have to wait for tensor memory
   static constexpr int kAsked = kBlocks == 4 ? 47 * 1024 : 78 * 1024;
+  static_assert(kStages * (kTile + kCodes) + 1024 <= kAsked, "the ring");
 };
 
 template <int NV>
@@ -119,6 +122,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<NV, GROUP>::kBlocks)) q4_tens
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  uint8_t* const codes_at = x_at + kStages * S::kTile;
   const uint32_t tmem = tmem_at, own_lanes = (uint32_t)(warp * 32) << 16, sums_at = tmem + 2 * kLeft;
 
   const int64_t q0 = (int64_t)blockIdx.y * NV;
@@ -127,41 +131,43 @@ __global__ void __launch_bounds__(kThreads, (Shape<NV, GROUP>::kBlocks)) q4_tens
   const int mine = (int)blockIdx.x < tiles ? (tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
   const int64_t total = (int64_t)mine * a.steps;
 
-  // The codes of two steps: this lane's half of its own row and of its neighbour's.  Rows behind the last repeat it; bytes behind a row's end are
-  // zeros, whose columns of the vectors are zero.
-  const int half = lane & 1, first = threadIdx.x & ~1;
-  int f_tile = blockIdx.x, f_step = 0;
+  // Codes and vectors of one step after the other: this lane's half of its own row and of its neighbour's, its pieces of the vectors' tile.  Rows
+  // behind the last repeat it; bytes behind a row's end are zeros, whose columns of the vectors are zero.
+  const int half = lane & 1;
+  int f_tile = blockIdx.x, f_step = 0, f_slot = 0;
   const uint8_t* f_src[2];
   auto aim = [&]() {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) f_src[j] = a.codes + min((int64_t)f_tile * 128 + first + j, a.n - 1) * a.code_stride + half * 16;
+    for (int j = 0; j < 2; ++j)
+      f_src[j] = a.codes + min((int64_t)f_tile * 128 + (threadIdx.x & ~1) + j, a.n - 1) * a.code_stride + half * 16;
   };
   aim();
-  uint4 held[2][2];
-  auto fetch = [&](uint4 (&to)[2]) {
-    if (f_tile >= tiles) return;
-    const int have = a.row_bytes - f_step * 32 - half * 16;
+  const uint4* const x0 = a.x + (int64_t)blockIdx.y * a.steps * (NV * 8) + threadIdx.x;
+  const uint32_t to_codes = smem_u32(codes_at) + threadIdx.x * 16, to_x = smem_u32(x_at) + threadIdx.x * 16;
+  auto fetch = [&]() {
+    if (f_tile < tiles) {
+      const int have = max(0, min(16, a.row_bytes - f_step * 32 - half * 16));
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if (have >= 16) {
-        to[j] = *VSK_CHK(reinterpret_cast<const uint4*>(f_src[j]));
-      } else {
-        uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int b = 0; b < 15; ++b)
-          if (b < have) w[b >> 2] |= (uint32_t)*VSK_CHK(f_src[j] + b) << (8 * (b & 3));
-        to[j] = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int j = 0; j < 2; ++j) {
+#ifdef VSK_CHECKED
+        const void* src = have == 16 ? (const void*)VSK_CHK((const uint4*)f_src[j]) : have ? (const void*)f_src[j] : a.codes;
+#else
+        const void* src = f_src[j];   // (of a copy of no bytes nothing is read)
+#endif
+        copy16(to_codes + f_slot * kCodes + j * (2048 + 16), src, have);
+        f_src[j] += 32;
       }
-      f_src[j] += 32;
+#pragma unroll
+      for (int j = 0; j < NV / 16; ++j) copy16(to_x + f_slot * S::kTile + j * (kThreads * 16), VSK_CHK(x0 + (int64_t)f_step * (NV * 8) + j * kThreads), 16);
+      f_slot = f_slot + 1 == kStages ? 0 : f_slot + 1;
+      if (++f_step == a.steps) {
+        f_step = 0;
+        f_tile += gridDim.x;
+        aim();
+      }
     }
-    if (++f_step == a.steps) {
-      f_step = 0;
-      f_tile += gridDim.x;
-      aim();
-    }
+    copy_commit();   // (an empty group keeps the count of groups in step)
   };
-  fetch(held[0]);
-  fetch(held[1]);
 
   // the scales of this thread's row, four groups at a time, the next four under way
   int s_tile = blockIdx.x, s_group = 0;
@@ -192,15 +198,8 @@ __global__ void __launch_bounds__(kThreads, (Shape<NV, GROUP>::kBlocks)) q4_tens
   for (int q = 0; q < NV; ++q) tot[q] = 0.f;
 
   wait_for_launches_before();   // x
-  const uint4* const x0 = a.x + (int64_t)blockIdx.y * a.steps * (NV * 8) + threadIdx.x;
-  uint4 xs[NV / 16];
-  int x_step = 0;
-  auto fetch_x = [&]() {
-#pragma unroll
-    for (int j = 0; j < NV / 16; ++j) xs[j] = *VSK_CHK(x0 + (int64_t)x_step * (NV * 8) + j * kThreads);
-    x_step = x_step + 1 == a.steps ? 0 : x_step + 1;
-  };
-  fetch_x();
+#pragma unroll 1
+  for (int s = 0; s < kStages - 1; ++s) fetch();
 
   bool ok = true;
   int group = 0;              // of the row: the next one whose sums are taken
@@ -241,30 +240,29 @@ __global__ void __launch_bounds__(kThreads, (Shape<NV, GROUP>::kBlocks)) q4_tens
   constexpr uint32_t kInstruction = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(NV >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
   int step = 0;
   int64_t tile = blockIdx.x;
-  auto body = [&](int64_t at, auto which) {
-    constexpr int B = decltype(which)::value;
+  int slot = 0;
+#pragma unroll 1
+  for (int64_t at = 0; at < total; ++at) {
+    const int b = (int)(at & 1);
+    copy_wait<kStages - 2>();
+    __syncwarp();
     {
-      const uint4 mine_of = half ? held[B][1] : held[B][0], other = half ? held[B][0] : held[B][1];
-      const uint32_t kept[4] = {mine_of.x, mine_of.y, mine_of.z, mine_of.w}, given[4] = {other.x, other.y, other.z, other.w};
+      const uint4* own = reinterpret_cast<const uint4*>(codes_at + slot * kCodes + (lane & 1) * (2048 + 16) + (threadIdx.x & ~1) * 16);
       uint32_t p[32];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t got = __shfl_xor_sync(0xffffffffu, given[i], 1);
-        uint32_t lo[4], hi[4];
-        unpack<T>(half ? got : kept[i], lo);
-        unpack<T>(half ? kept[i] : got, hi);
+      for (int h = 0; h < 2; ++h) {
+        const uint4 v = own[h];
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          p[i * 4 + e] = lo[e];
-          p[16 + i * 4 + e] = hi[e];
+        for (int i = 0; i < 4; ++i) {
+          uint32_t four[4];
+          unpack<T>(w[i], four);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[h * 16 + i * 4 + e] = four[e];
         }
       }
-      store_codes(tmem + own_lanes + B * kLeft, p);
+      store_codes(tmem + own_lanes + b * kLeft, p);
     }
-#pragma unroll
-    for (int j = 0; j < NV / 16; ++j) *reinterpret_cast<uint4*>(x_at + B * S::kTile + (threadIdx.x + j * kThreads) * 16) = xs[j];
-    fetch(held[B]);
-    fetch_x();
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
     tc_fence_before();
@@ -272,19 +270,21 @@ __global__ void __launch_bounds__(kThreads, (Shape<NV, GROUP>::kBlocks)) q4_tens
     if (warp == 0) {
       tc_fence_after();
       if (elect_one() && ok) {
-        const uint32_t lo_b = desc_lo(smem_u32(x_at + B * S::kTile)), to = sums_at + (issued & 1) * (NV * S::kPer);
+        const uint32_t lo_b = desc_lo(smem_u32(x_at + slot * S::kTile)), to = sums_at + (issued & 1) * (NV * S::kPer);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const uint32_t more = GROUP == 128 ? (uint32_t)(k > 0 || (step & 1)) : GROUP == 64 ? (uint32_t)(k > 0) : (uint32_t)(k & 1);
-          multiply(GROUP == 32 ? to + (k >> 1) * NV : to, tmem + B * kLeft + k * 8, desc_pack(lo_b + k * 2, kDescHi), kInstruction, more);
+          multiply(GROUP == 32 ? to + (k >> 1) * NV : to, tmem + b * kLeft + k * 8, desc_pack(lo_b + k * 2, kDescHi), kInstruction, more);
         }
-        tc_commit(&done[B]);
+        tc_commit(&done[b]);
       }
       __syncwarp();
     }
     if (step > 0) finish(at - 1, ends_group(step - 1));
+    fetch();   // into the stage of the step before, whose products are done
+    slot = slot + 1 == kStages ? 0 : slot + 1;
     if (ends_group(step)) ++issued;
-    if (++step < a.steps) return;
+    if (++step < a.steps) continue;
     // the tile's end: the last step's sums, and the results
     finish(at, true);
     const int64_t row = tile * 128 + threadIdx.x;
@@ -307,11 +307,6 @@ __global__ void __launch_bounds__(kThreads, (Shape<NV, GROUP>::kBlocks)) q4_tens
     group = 0;
     step = 0;
     tile += gridDim.x;
-  };
-#pragma unroll 1
-  for (int64_t at = 0; at < total; at += 2) {
-    body(at, std::integral_constant<int, 0>());
-    if (at + 1 < total) body(at + 1, std::integral_constant<int, 1>());
   }
   if (!ok) {
     gave_up = 1;
