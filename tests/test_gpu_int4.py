@@ -182,24 +182,25 @@ def test_products_with_rows_inside_wider_ones(dev, kind, code_pad, scale_pad, x_
 
 
 # rows enough to fill the machine, at 16-byte places: one tile of 128 rows to a block and several, ends inside a tile, one step of 64 columns,
-# odd numbers of steps, ends inside a group, vectors of more than one pass
-@pytest.mark.parametrize("n,dim,nq", [(18_944, 64, 5), (19_073, 129, 17), (20_001, 200, 16), (40_000, 1000, 32), (152_000, 65, 40), (80_001, 321, 9)])
+# odd numbers of steps, ends inside a group, vectors of more than one pass; and up to sixteen vectors with as many rows
+@pytest.mark.parametrize("n,dim,nq", [(18_944, 64, 17), (19_073, 129, 32), (9_601, 200, 61), (40_000, 1000, 32), (152_000, 65, 40), (80_001, 321, 9),
+                                      (30, 1100, 4_760)])
 @pytest.mark.parametrize("group", [32, 64, 128])
-@pytest.mark.parametrize("kind", ["f16", "bf16"])
-def test_products_with_many_rows(dev, kind, group, n, dim, nq):
+@pytest.mark.parametrize("kind,symmetric", [("f16", False), ("bf16", True)])
+def test_products_with_many_rows(dev, kind, symmetric, group, n, dim, nq):
     import torch
     rng = np.random.default_rng(n + dim + nq + group)
-    codes, scales, _ = _case(rng, n, dim, group, True)
+    codes, scales, middles = _case(rng, n, dim, group, symmetric)
     x = torch.from_numpy(rng.standard_normal((nq, dim))).to(_t(kind))
     width, groups = (dim + 1) // 2, scales.shape[1]
-    for out, scale_pad in ((kind, -groups % 4), ("f32", 1)):
-        _compare(_run(dev, codes, scales, None, group, x, out, code_pad=-width % 16, scale_pad=scale_pad), codes, scales, None, group, x, out)
+    out, scale_pad = ((kind, -groups % 4), ("f32", 1))[(n + group) // 32 % 2]
+    _compare(_run(dev, codes, scales, middles, group, x, out, code_pad=-width % 16, scale_pad=scale_pad), codes, scales, middles, group, x, out)
     bad = x.clone()
     bad[nq // 2, dim - 1] = float("inf")
-    got = _run(dev, codes, scales, None, group, bad, "f32", code_pad=-width % 16)
+    got = _run(dev, codes, scales, middles, group, bad, "f32", code_pad=-width % 16)
     others = np.arange(nq) != nq // 2
     assert not np.isfinite(got[nq // 2]).any()
-    assert np.array_equal(got[others], _run(dev, codes, scales, None, group, x, "f32", code_pad=-width % 16)[others])
+    assert np.array_equal(got[others], _run(dev, codes, scales, middles, group, x, "f32", code_pad=-width % 16)[others])
 
 
 def test_products_of_unusual_vectors(dev):

@@ -18,7 +18,7 @@ int32_t q4_product(Ctx* ctx, const vsk_q4_rows& rows, const void* x, int32_t x_d
 int32_t q4_product_digits(Ctx* ctx, const vsk_q4_rows& rows, const void* x, int32_t x_dtype, int64_t nq, int64_t x_stride, void* y,
                           int32_t y_dtype, int64_t y_stride);
 
-// The same on the tensor cores' block form, for rows without middles, at 16-byte places, that fill the machine (int4_tensor.cu).
+// The same on the tensor cores' block form, for more than 16 vectors and rows at 16-byte places that fill the machine (int4_tensor.cu).
 bool q4_fits_tensor(Ctx* ctx, const vsk_q4_rows& rows, int64_t nq);
 int32_t q4_product_tensor(Ctx* ctx, const vsk_q4_rows& rows, const void* x, int32_t x_dtype, int64_t nq, int64_t x_stride, void* y,
                           int32_t y_dtype, int64_t y_stride);

@@ -5,7 +5,7 @@
 // plus the code, and taking the power and 8 away needs no rounding.  A group's sum is taken in fp32 registers, multiplied by the
 // scale there and added to the row's total: codes are never multiplied by a rounded weight.
 //
-// Rows that fill the machine at 16-byte places, without middles, go to int4_tensor.cu.  131 072 x 2 048, groups of 128, 32 bf16 vectors, here: 104 us,
+// More than 16 vectors, with rows that fill the machine at 16-byte places, go to int4_tensor.cu.  131 072 x 2 048, groups of 128, 32 bf16 vectors, here: 104 us,
 // where the warp form's rate would allow 31: tensor pipe 33 %, issue slots 32 %, each warp alternating between unpacking and products.  Four tiles
 // of rows per warp, 2 - 6 stages, two blocks per SM, sixteen warps in step with x in shared memory were all within 7 %.
 //

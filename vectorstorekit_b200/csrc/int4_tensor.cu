@@ -2,7 +2,7 @@
 //
 // A wait that runs out ends the block's part with what it has: the call returns VSK_ERR_TIMEOUT.
 //
-// A block takes 128 rows (the matrix instruction's M) and NV = 16 or 32 vectors (its N).  Per step of 64 columns
+// A block takes 128 rows (the matrix instruction's M) and NV = 32 vectors (its N).  Per step of 64 columns
 //   codes     32 bytes per row, copied to a warp's part of a ring by two lanes a row, four steps ahead; a thread takes its row's, which become exact
 //             16-bit numbers (code - 8) in tensor memory, the instruction's left side.  A word of eight codes is four columns there, in the
 //             order 0 4 1 5 2 6 3 7, which the vectors' tile has too
@@ -10,10 +10,13 @@
 //             is copied to the ring as it is
 //   products  four instructions of 16 columns, sums of one group of columns per accumulator in tensor memory
 //   scales    a thread owns a row: it reads the group's sums of its row, multiplies by the scale in fp32 and adds to the row's NV totals, while
-//             the next step's products run.  Accumulators, operands and barriers are double
+//             the next step's products run; middles likewise, times the vectors' sums over the group, which come with the step's copies.
+//             Accumulators, operands and barriers are double
 // Codes are never multiplied by a rounded weight: every product is exact, sums are fp32.
 //
-// 131 072 x 2 048, groups of 128, 32 bf16 vectors: the call takes 84 us, 127 with the warp form.
+// 131 072 x 2 048, groups of 128, 32 bf16 vectors: the call takes 84 us, 127 with the warp form.  Bound by a step's chain (copies - numbers - tensor
+// memory - products - sums, about 0.6 us for a block alone, four blocks to an SM) and by 1 024 tiles on 592 blocks.  Codes to shared memory
+// instead of tensor memory: 97 against 93 us, then codes and vectors asked for through registers two and one steps ahead instead of copies: 93 against 84.
 #include "int4.cuh"
 #include "tc_ptx.cuh"
 
@@ -21,8 +24,9 @@ namespace vsk {
 namespace {
 using namespace tc;
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 128, NV = 32;
 constexpr int kStages = 5;
+constexpr int kSumStages = kStages + 1;   // of the vectors' sums, which other threads may still read when the next copies begin
 constexpr int kCodes = 4096 + 16;   // of a stage: even rows, 16 bytes, odd rows (so that the rows of a read lie in different banks)
 constexpr int kLeft = 32;           // columns of tensor memory that a step's codes take: 64 numbers of 16 bits
 
@@ -31,11 +35,13 @@ struct TensorArgs {
   const uint8_t* codes;
   int64_t code_stride;
   const __half* scales;
+  const __half* middles;          // or null
   int64_t scale_stride;
   int64_t n;
   int row_bytes, groups, steps;   // steps of 64 columns
   int quads;                      // four scales of a row can be read at once
   const uint4* x;                 // [chunk][step][NV][8 pieces, turned]
+  const float* sums;              // [chunk][group][NV]: sums of x over the groups, if there are middles
   int64_t nq;
   void* y;
   int64_t y_stride;
@@ -43,31 +49,17 @@ struct TensorArgs {
   int* err;                       // pinned: a wait ran out
 };
 
-template <int NV, int GROUP>
+template <int GROUP>
 struct Shape {
   static constexpr int kPer = GROUP == 32 ? 2 : 1;                         // groups that end in a step, at most
-  static constexpr int kSums = 2 * NV * kPer;                              // columns of tensor memory: 32, 64 or 128, behind two steps' codes
+  static constexpr int kSums = 2 * NV * kPer;                              // columns of tensor memory, 64 or 128, behind two steps' codes
   static constexpr int kColumns = 2 * kLeft + kSums <= 128 ? 128 : 256;
   static constexpr int kBlocks = 512 / kColumns;                           // per SM
   static constexpr int kTile = NV * 128;
   // so much that no further block would have to wait for tensor memory
   static constexpr int kAsked = kBlocks == 4 ? 47 * 1024 : 78 * 1024;
-  static_assert(kStages * (kTile + kCodes) + 1024 <= kAsked, "the ring");
+  static_assert(kStages * (kTile + kCodes) + kSumStages * kPer * NV * 4 + 1024 <= kAsked, "the ring");
 };
-
-template <int NV>
-__device__ __forceinline__ void load_sums(uint32_t at, float (&v)[NV]) {
-  if constexpr (NV == 32) {
-    tc_ld32(at, v);
-  } else {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
-                   "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
-                 : "r"(at)
-                 : "memory");
-    tc_ld_wait();
-  }
-}
 
 // 32 columns of this thread's lane; done behind a tcgen05.wait::st.
 __device__ __forceinline__ void store_codes(uint32_t at, const uint32_t (&r)[32]) {
@@ -91,6 +83,12 @@ __device__ __forceinline__ void multiply(uint32_t sums, uint32_t left, uint64_t 
       : "memory");
 }
 
+__device__ __forceinline__ void add_pair(float& a, float& b, float by, float x, float y) {
+  const float2 r = __ffma2_rn(make_float2(by, by), make_float2(x, y), make_float2(a, b));
+  a = r.x;
+  b = r.y;
+}
+
 // False when the limit of looks has run out.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) {
   for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
@@ -100,9 +98,9 @@ __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) {
   return false;
 }
 
-template <typename T, int NV, int GROUP>
-__global__ void __launch_bounds__(kThreads, (Shape<NV, GROUP>::kBlocks)) q4_tensor_kernel(const __grid_constant__ TensorArgs a) {
-  using S = Shape<NV, GROUP>;
+template <typename T, int GROUP, bool MID>
+__global__ void __launch_bounds__(kThreads, (Shape<GROUP>::kBlocks)) q4_tensor_kernel(const __grid_constant__ TensorArgs a) {
+  using S = Shape<GROUP>;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t done[2];
   __shared__ uint32_t tmem_at;
@@ -123,6 +121,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<NV, GROUP>::kBlocks)) q4_tens
   __syncthreads();
   tc_fence_after();
   uint8_t* const codes_at = x_at + kStages * S::kTile;
+  float* const sums_of = reinterpret_cast<float*>(codes_at + kStages * kCodes);   // [kSumStages][groups of a step][NV]
   const uint32_t tmem = tmem_at, own_lanes = (uint32_t)(warp * 32) << 16, sums_at = tmem + 2 * kLeft;
 
   const int64_t q0 = (int64_t)blockIdx.y * NV;
@@ -134,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<NV, GROUP>::kBlocks)) q4_tens
   // Codes and vectors of one step after the other: this lane's half of its own row and of its neighbour's, its pieces of the vectors' tile.  Rows
   // behind the last repeat it; bytes behind a row's end are zeros, whose columns of the vectors are zero.
   const int half = lane & 1;
-  int f_tile = blockIdx.x, f_step = 0, f_slot = 0;
+  int f_tile = blockIdx.x, f_step = 0, f_slot = 0, f_sums = 0;
   const uint8_t* f_src[2];
   auto aim = [&]() {
 #pragma unroll
@@ -159,6 +158,13 @@ __global__ void __launch_bounds__(kThreads, (Shape<NV, GROUP>::kBlocks)) q4_tens
       }
 #pragma unroll
       for (int j = 0; j < NV / 16; ++j) copy16(to_x + f_slot * S::kTile + j * (kThreads * 16), VSK_CHK(x0 + (int64_t)f_step * (NV * 8) + j * kThreads), 16);
+      if constexpr (MID) {
+        const int e = threadIdx.x / (NV / 4), g = GROUP == 32 ? 2 * f_step + e : GROUP == 64 ? f_step : f_step >> 1;
+        if (e < S::kPer && g < a.groups)
+          copy16(smem_u32(sums_of + f_sums * (S::kPer * NV)) + threadIdx.x * 16,
+                 VSK_CHK(reinterpret_cast<const uint4*>(a.sums + ((int64_t)blockIdx.y * a.groups + g) * NV) + threadIdx.x % (NV / 4)), 16);
+        f_sums = f_sums + 1 == kSumStages ? 0 : f_sums + 1;
+      }
       f_slot = f_slot + 1 == kStages ? 0 : f_slot + 1;
       if (++f_step == a.steps) {
         f_step = 0;
@@ -169,20 +175,28 @@ __global__ void __launch_bounds__(kThreads, (Shape<NV, GROUP>::kBlocks)) q4_tens
     copy_commit();   // (an empty group keeps the count of groups in step)
   };
 
-  // the scales of this thread's row, four groups at a time, the next four under way
+  // the scales (and middles) of this thread's row, four groups at a time, the next four under way
+  struct Four {
+    uint2 s, m;
+    __device__ __forceinline__ static float of(uint2 v, int group) {
+      const uint32_t pair = (group & 2) ? v.y : v.x;
+      return __half2float(__ushort_as_half((unsigned short)((group & 1) ? pair >> 16 : pair)));
+    }
+  };
   int s_tile = blockIdx.x, s_group = 0;
-  auto scales_of_four = [&]() {
-    uint2 v = make_uint2(0, 0);
-    if (s_tile < tiles) {
-      const __half* at = a.scales + min((int64_t)s_tile * 128 + threadIdx.x, a.n - 1) * a.scale_stride + s_group;
-      if (a.quads && s_group + 4 <= a.groups) {
-        v = *VSK_CHK(reinterpret_cast<const uint2*>(at));
-      } else {
-        uint32_t h[4];
+  auto four = [&](const __half* at) {
+    if (a.quads && s_group + 4 <= a.groups) return *VSK_CHK(reinterpret_cast<const uint2*>(at));
+    uint32_t h[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) h[e] = s_group + e < a.groups ? __half_as_ushort(*VSK_CHK(at + e)) : 0;
-        v = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
-      }
+    for (int e = 0; e < 4; ++e) h[e] = s_group + e < a.groups ? __half_as_ushort(*VSK_CHK(at + e)) : 0;
+    return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+  };
+  auto next_four = [&]() {
+    Four v{};
+    if (s_tile < tiles) {
+      const int64_t at = min((int64_t)s_tile * 128 + threadIdx.x, a.n - 1) * a.scale_stride + s_group;
+      v.s = four(a.scales + at);
+      if constexpr (MID) v.m = four(a.middles + at);
       s_group += 4;
       if (s_group >= a.groups) {
         s_group = 0;
@@ -191,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, (Shape<NV, GROUP>::kBlocks)) q4_tens
     }
     return v;
   };
-  uint2 scales = make_uint2(0, 0), scales_next = scales_of_four();
+  Four now{}, next = next_four();
 
   float tot[NV];
 #pragma unroll
@@ -203,30 +217,38 @@ __global__ void __launch_bounds__(kThreads, (Shape<NV, GROUP>::kBlocks)) q4_tens
 
   bool ok = true;
   int group = 0;              // of the row: the next one whose sums are taken
+  int sums_now = 0;           // the stage of the step's sums of vectors
   int issued = 0, taken = 0;  // groups so far: their accumulators alternate
   // The sums of the step before `at` steps: waits for its products, and takes the groups that ended with them.
   auto finish = [&](int64_t at, bool ends) {
     if (ok) ok = wait_for(&done[at & 1], (uint32_t)(at >> 1) & 1u);
     __syncwarp();
     tc_fence_after();
+    const int sum_slot = sums_now;
+    if constexpr (MID) sums_now = sums_now + 1 == kSumStages ? 0 : sums_now + 1;
     if (!ends) return;
     const uint32_t from = sums_at + own_lanes + (taken & 1) * (NV * S::kPer);
 #pragma unroll
     for (int e = 0; e < S::kPer; ++e) {
       float v[NV];
-      load_sums<NV>(from + e * NV, v);
+      tc_ld32(from + e * NV, v);
       if ((group & 3) == 0) {
-        scales = scales_next;
-        scales_next = scales_of_four();
+        now = next;
+        next = next_four();
       }
-      const uint32_t pair = (group & 2) ? scales.y : scales.x;
-      const float s = __half2float(__ushort_as_half((unsigned short)((group & 1) ? pair >> 16 : pair)));
       if (group < a.groups) {
+        const float s = Four::of(now.s, group);
 #pragma unroll
-        for (int q = 0; q < NV; q += 2) {
-          const float2 r = __ffma2_rn(make_float2(s, s), make_float2(v[q], v[q + 1]), make_float2(tot[q], tot[q + 1]));
-          tot[q] = r.x;
-          tot[q + 1] = r.y;
+        for (int q = 0; q < NV; q += 2) add_pair(tot[q], tot[q + 1], s, v[q], v[q + 1]);
+        if constexpr (MID) {
+          const float m = Four::of(now.m, group);
+          const float4* x = reinterpret_cast<const float4*>(sums_of + sum_slot * (S::kPer * NV) + e * NV);
+#pragma unroll
+          for (int q = 0; q < NV; q += 4) {
+            const float4 xs = x[q / 4];
+            add_pair(tot[q], tot[q + 1], m, xs.x, xs.y);
+            add_pair(tot[q + 2], tot[q + 3], m, xs.z, xs.w);
+          }
         }
         ++group;
       }
@@ -321,26 +343,33 @@ __global__ void __launch_bounds__(kThreads, (Shape<NV, GROUP>::kBlocks)) q4_tens
   }
 }
 
-// x as the steps' tiles, zeros behind dim and behind the last vector: a thread per eight columns of one vector.
+// x as the steps' tiles, zeros behind dim and behind the last vector, and its sums over the groups: a thread per eight columns of one vector.
 template <typename T>
 __global__ void __launch_bounds__(128) q4_to_tiles_kernel(const T* __restrict__ x, int64_t x_stride, int64_t nq, int64_t q_first, int dim, int steps,
-                                                          int nv, uint4* __restrict__ out) {
+                                                          int group, int groups, uint4* __restrict__ out, float* __restrict__ sums) {
   let_the_next_launch_begin();
   const int64_t q = q_first + blockIdx.y;
   const int p = blockIdx.x * 128 + threadIdx.x, col = p * 8;
-  if (p >= steps * 8) return;
   __align__(16) T v[8];
+  float s = 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = q < nq && col + j < dim ? *VSK_CHK(x + q * x_stride + col + j) : T(0.f);
+  for (int j = 0; j < 8; ++j) {
+    v[j] = q < nq && col + j < dim ? *VSK_CHK(x + q * x_stride + col + j) : T(0.f);
+    s += (float)v[j];
+  }
+  for (int o = group / 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int64_t chunk = q / NV;
+  const int c = (int)(q % NV);
+  if (sums && col % group == 0 && col < dim) *VSK_CHK_W(sums + (chunk * groups + col / group) * NV + c) = s;
+  if (p >= steps * 8) return;
   __align__(16) T w[8] = {v[0], v[4], v[1], v[5], v[2], v[6], v[3], v[7]};   // as the codes of a word are taken apart
-  const int c = (int)(q % nv);
-  *VSK_CHK_W(out + ((q / nv * steps + (p >> 3)) * nv + c) * 8 + ((p & 7) ^ (c & 7))) = *reinterpret_cast<const uint4*>(w);
+  *VSK_CHK_W(out + ((chunk * steps + (p >> 3)) * NV + c) * 8 + ((p & 7) ^ (c & 7))) = *reinterpret_cast<const uint4*>(w);
 }
 
-template <typename T, int NV, int GROUP>
+template <typename T, int GROUP, bool MID>
 int32_t launch(Ctx* ctx, const TensorArgs& a) {
-  using S = Shape<NV, GROUP>;
-  auto kernel = q4_tensor_kernel<T, NV, GROUP>;
+  using S = Shape<GROUP>;
+  auto kernel = q4_tensor_kernel<T, GROUP, MID>;
   VSK_CUDA(ctx, opt_in_shared(ctx, kernel, S::kAsked));
   const int64_t chunks = ceil_div(a.nq, NV), tiles = ceil_div(a.n, 128);
   const int64_t blocks = std::min(tiles, std::max<int64_t>(1, (int64_t)ctx->prop.multiProcessorCount * S::kBlocks / chunks));
@@ -359,26 +388,32 @@ int32_t launch(Ctx* ctx, const TensorArgs& a) {
   return VSK_OK;
 }
 
+template <typename T, int GROUP>
+int32_t by_middles(Ctx* ctx, const TensorArgs& a) {
+  return a.middles ? launch<T, GROUP, true>(ctx, a) : launch<T, GROUP, false>(ctx, a);
+}
 template <typename T>
-int32_t prepare_and_launch(Ctx* ctx, const TensorArgs& a, const T* x, int64_t x_stride, int dim, int group, int nv) {
-  const int64_t vectors = ceil_div(a.nq, nv) * nv;
+int32_t prepare_and_launch(Ctx* ctx, const TensorArgs& a, const T* x, int64_t x_stride, int dim, int group) {
+  const int64_t vectors = ceil_div(a.nq, NV) * NV;
   for (int64_t q = 0; q < vectors; q += 65535) {
     q4_to_tiles_kernel<T><<<dim3((unsigned)ceil_div(a.steps * 8, 128), (unsigned)std::min<int64_t>(65535, vectors - q)), 128, 0, ctx->stream>>>(
-        x, x_stride, a.nq, q, dim, a.steps, nv, (uint4*)a.x);
+        x, x_stride, a.nq, q, dim, a.steps, group, a.groups, (uint4*)a.x, (float*)a.sums);
     ctx->stats.kernel_launches++;
     VSK_CUDA(ctx, cudaGetLastError());
   }
-  if (nv == 16) return group == 32 ? launch<T, 16, 32>(ctx, a) : group == 64 ? launch<T, 16, 64>(ctx, a) : launch<T, 16, 128>(ctx, a);
-  return group == 32 ? launch<T, 32, 32>(ctx, a) : group == 64 ? launch<T, 32, 64>(ctx, a) : launch<T, 32, 128>(ctx, a);
+  return group == 32 ? by_middles<T, 32>(ctx, a) : group == 64 ? by_middles<T, 64>(ctx, a) : by_middles<T, 128>(ctx, a);
 }
 
 }  // namespace
 
-// A tile of 128 rows for every SM: with fewer the warp form, which shares a tile's columns among warps, fills the machine better.
+// More than 16 vectors, and a tile of 128 rows and 32 vectors for every SM: warp form / this one, us, symmetric: 19 000 x 4 096, 32 vectors 56 / 57;
+// 28 000 63 / 60; 152 000 229 / 161; 10 000 x 1 024, 64 vectors 35 / 28; 4 000 x 512, 200 vectors 29 / 24; fewer: 10 000 x 4 096, 32 vectors
+// 44 / 56.  Middles: 152 000 x 2 048, groups of 128, 32 vectors 158 / 102; 152 000 x 148, groups of 32: 75 / 43.  Groups of 32 have two blocks to an SM
+// (accumulators of both of a step's groups, double): 152 000 x 4 096, 17 vectors 240 / 246.  Up to 16 vectors the warp form does half the work and this one the same: 152 000 x 4 096, 16 vectors, groups of 32: 154 / 177.
 bool q4_fits_tensor(Ctx* ctx, const vsk_q4_rows& rows, int64_t nq) {
   const uintptr_t code_bits = reinterpret_cast<uintptr_t>(rows.codes) | (uintptr_t)rows.code_stride;
-  return !rows.middles && (code_bits & 15) == 0 && rows.n >= 128 * (int64_t)ctx->prop.multiProcessorCount && ceil_div(rows.n, 128) < (1 << 30) &&
-         nq <= 16 * 65535;
+  const int64_t tiles = ceil_div(rows.n, 128), chunks = ceil_div(nq, NV);
+  return nq > 16 && (code_bits & 15) == 0 && tiles < (1 << 30) && chunks <= 65535 && tiles * chunks >= ctx->prop.multiProcessorCount;
 }
 
 int32_t q4_product_tensor(Ctx* ctx, const vsk_q4_rows& rows, const void* x, int32_t x_dtype, int64_t nq, int64_t x_stride, void* y,
@@ -392,21 +427,24 @@ int32_t q4_product_tensor(Ctx* ctx, const vsk_q4_rows& rows, const void* x, int3
   a.row_bytes = (rows.dim + 1) / 2;
   a.groups = (int)ceil_div(rows.dim, rows.group);
   a.steps = (int)ceil_div(rows.dim, 64);
-  a.quads = ((reinterpret_cast<uintptr_t>(rows.scales) | (uintptr_t)(2 * rows.scale_stride)) & 7) == 0;
+  a.middles = (const __half*)rows.middles;
+  a.quads = ((reinterpret_cast<uintptr_t>(rows.scales) | reinterpret_cast<uintptr_t>(rows.middles) | (uintptr_t)(2 * rows.scale_stride)) & 7) == 0;
   a.nq = nq;
   a.y = y;
   a.y_stride = y_stride;
   a.y_dtype = y_dtype;
-  const int nv = nq <= 16 ? 16 : 32;
+  const int64_t vectors = ceil_div(nq, NV) * NV;
+  const size_t tile_bytes = (size_t)vectors * a.steps * 128, sum_bytes = rows.middles ? (size_t)vectors * a.groups * 4 : 0;
   void* p;
-  VSK_TRY(scratch(ctx, SLOT_Q16, (size_t)ceil_div(nq, nv) * nv * a.steps * 128, &p));
+  VSK_TRY(scratch(ctx, SLOT_Q16, tile_bytes + sum_bytes, &p));
   a.x = (const uint4*)p;
+  a.sums = sum_bytes ? (const float*)((uint8_t*)p + tile_bytes) : nullptr;
   VSK_TRY(pinned_reserve(ctx, &ctx->host_flags[0], sizeof(int)));
   volatile int* gave_up = (volatile int*)ctx->host_flags[0].p;
   *gave_up = 0;
   a.err = (int*)ctx->host_flags[0].p;
-  VSK_TRY(x_dtype == VSK_DTYPE_F16 ? prepare_and_launch(ctx, a, (const __half*)x, x_stride, rows.dim, rows.group, nv)
-                                   : prepare_and_launch(ctx, a, (const __nv_bfloat16*)x, x_stride, rows.dim, rows.group, nv));
+  VSK_TRY(x_dtype == VSK_DTYPE_F16 ? prepare_and_launch(ctx, a, (const __half*)x, x_stride, rows.dim, rows.group)
+                                   : prepare_and_launch(ctx, a, (const __nv_bfloat16*)x, x_stride, rows.dim, rows.group));
   tl_mark(ctx, "q4_product");
   VSK_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
   if (*gave_up) return fail(ctx, VSK_ERR_TIMEOUT, "products with rows in four bits: a bounded wait ran out");
