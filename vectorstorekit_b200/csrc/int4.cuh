@@ -34,6 +34,34 @@ template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.
 __device__ __forceinline__ void wait_for_launches_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_the_next_launch_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// The vectors as the caller has them, for products that are taken one by one.
+struct Vectors {
+  const void* x;
+  int64_t stride;
+  int dtype;
+  __device__ __forceinline__ float at(int64_t q, int64_t column) const {
+    const int64_t e = q * stride + column;
+    if (dtype == VSK_DTYPE_F32) return *VSK_CHK((const float*)x + e);
+    if (dtype == VSK_DTYPE_F16) return __half2float(*VSK_CHK((const __half*)x + e));
+    return __bfloat162float(*VSK_CHK((const __nv_bfloat16*)x + e));
+  }
+};
+
+// The product of one row with a vector that holds an infinity or a NaN, from the definition: each value s (c - 8) + m first.  (The sums of
+// s (c - 8) x and of m x are two infinities that need not agree, or 0 times one.)
+template <typename Args>
+__device__ __noinline__ float plain_product(const Args& a, const Vectors& x, int64_t row, int64_t q) {
+  float sum = 0.f;
+  for (int i = 0; i < a.dim; ++i) {
+    const uint8_t b = *VSK_CHK(a.codes + row * a.code_stride + (i >> 1));
+    const int c = (int)((i & 1) ? b >> 4 : b & 15) - 8;
+    float v = __half2float(*VSK_CHK(a.scales + row * a.scale_stride + i / a.group)) * (float)c;
+    if (a.middles) v += __half2float(*VSK_CHK(a.middles + row * a.scale_stride + i / a.group));
+    sum = fmaf(v, x.at(q, i), sum);
+  }
+  return sum;
+}
+
 __device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t bits) {   // (w & mask) | bits, in one instruction
   uint32_t r;
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));

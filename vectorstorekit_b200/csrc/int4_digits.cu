@@ -51,9 +51,7 @@ struct DigitArgs {
   const float* sums;          // [vector][sum_stride]: sums of x over the groups (zeros behind the last)
   int sum_stride;
   const VectorInfo* info;     // [vector]
-  const void* x;              // for vectors that are not finite
-  int64_t x_stride;
-  int x_dtype;
+  Vectors x;                  // for those that are not finite
   int64_t nq;
   int per_launch;             // vectors per grid row
   void* y;
@@ -89,29 +87,10 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
   return r;
 }
 
-__device__ __forceinline__ float x_at(const DigitArgs& a, int64_t at) {
-  if (a.x_dtype == VSK_DTYPE_F32) return *VSK_CHK((const float*)a.x + at);
-  if (a.x_dtype == VSK_DTYPE_F16) return __half2float(*VSK_CHK((const __half*)a.x + at));
-  return __bfloat162float(*VSK_CHK((const __nv_bfloat16*)a.x + at));
-}
-
 __device__ __forceinline__ void store_y(const DigitArgs& a, int64_t at, float v) {
   if (a.y_dtype == VSK_DTYPE_F32) *VSK_CHK_W((float*)a.y + at) = v;
   else if (a.y_dtype == VSK_DTYPE_F16) *VSK_CHK_W((__half*)a.y + at) = __float2half_rn(v);
   else *VSK_CHK_W((__nv_bfloat16*)a.y + at) = __float2bfloat16_rn(v);
-}
-
-// The product of one row with a vector that holds an infinity or a NaN.
-__device__ __noinline__ float plain_product(const DigitArgs& a, int64_t row, int64_t q) {
-  float sum = 0.f;
-  for (int i = 0; i < a.dim; ++i) {
-    const uint8_t b = *VSK_CHK(a.codes + row * a.code_stride + (i >> 1));
-    const int c = (int)((i & 1) ? b >> 4 : b & 15) - 8;
-    float v = __half2float(*VSK_CHK(a.scales + row * a.scale_stride + i / a.group)) * (float)c;
-    if (a.middles) v += __half2float(*VSK_CHK(a.middles + row * a.scale_stride + i / a.group));
-    sum = fmaf(v, x_at(a, q * a.x_stride + i), sum);
-  }
-  return sum;
 }
 
 __device__ __forceinline__ uint32_t masked_turned(uint32_t w) {   // (w & 0xf0f0f0f0) ^ 0x80808080, in one instruction
@@ -456,7 +435,7 @@ __global__ void __launch_bounds__(32 * kWarps, DT == 4 ? 1 : 2) q4_digits_kernel
       // (the digits' numbers are 16 times the products, and the last one added counts 256^3)
       v = ldexpf(v, exponent + 8 * (kDigits - 1) - 4) + m;
       if (row < a.n) {
-        if (exponent == INT_MIN) v = plain_product(a, row, q0 + q);
+        if (exponent == INT_MIN) v = plain_product(a, a.x, row, q0 + q);
         store_y(a, (q0 + q) * a.y_stride + row, v);
       }
     }
@@ -644,9 +623,7 @@ int32_t q4_product_digits(Ctx* ctx, const vsk_q4_rows& rows, const void* x, int3
   const int gw = 128 / rows.group;
   const uintptr_t scale_bits = reinterpret_cast<uintptr_t>(rows.scales) | reinterpret_cast<uintptr_t>(rows.middles) | (uintptr_t)(2 * rows.scale_stride);
   a.pair_scales = (scale_bits & (uintptr_t)(2 * gw - 1)) == 0;
-  a.x = x;
-  a.x_stride = x_stride;
-  a.x_dtype = x_dtype;
+  a.x = Vectors{x, x_stride, x_dtype};
   a.nq = nq;
   a.y = y;
   a.y_stride = y_stride;

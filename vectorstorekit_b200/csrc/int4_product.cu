@@ -37,6 +37,7 @@ struct ProductArgs {
   int pair_scales;            // a step's scales (and middles) of a row can be read at once
   const uint4* frags;         // [chunk][kstep][32 columns][tile of 8 vectors][32 lanes]
   const float* sums;          // [chunk][kstep * groups of it][8 * tiles]: sums of x over the groups
+  Vectors x;                  // for those that are not finite
   int64_t nq;
   int per_launch;             // vectors per grid row
   void* y;
@@ -331,7 +332,10 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 4 ? 1 : 2) q4_product_kerne
     for (int q = wk; q < nq; q += team) {
       float v = 0.f;
       for (int w = 0; w < team; ++w) v += red[(w * 32 + lane) * S::kLine + q];
-      if (row < a.n) store_y(a, (q0 + q) * a.y_stride + row, v);
+      if (row < a.n) {
+        if (MID && !isfinite(v)) v = plain_product(a, a.x, row, q0 + q);   // (without middles both orders answer alike)
+        store_y(a, (q0 + q) * a.y_stride + row, v);
+      }
     }
     meet();
   }
@@ -436,6 +440,7 @@ int32_t q4_product(Ctx* ctx, const vsk_q4_rows& rows, const void* x, int32_t x_d
   const int gw = 128 / rows.group;
   const uintptr_t scale_bits = reinterpret_cast<uintptr_t>(rows.scales) | reinterpret_cast<uintptr_t>(rows.middles) | (uintptr_t)(2 * rows.scale_stride);
   a.pair_scales = (scale_bits & (uintptr_t)(2 * gw - 1)) == 0;
+  a.x = Vectors{x, x_stride, x_dtype};
   a.nq = nq;
   a.y = y;
   a.y_stride = y_stride;

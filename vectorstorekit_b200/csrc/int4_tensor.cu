@@ -38,10 +38,12 @@ struct TensorArgs {
   const __half* middles;          // or null
   int64_t scale_stride;
   int64_t n;
+  int dim, group;
   int row_bytes, groups, steps;   // steps of 64 columns
   int quads;                      // four scales of a row can be read at once
   const uint4* x;                 // [chunk][step][NV][8 pieces, turned]
   const float* sums;              // [chunk][group][NV]: sums of x over the groups, if there are middles
+  Vectors vectors;                // for those that are not finite
   int64_t nq;
   void* y;
   int64_t y_stride;
@@ -322,6 +324,19 @@ __global__ void __launch_bounds__(kThreads, (Shape<GROUP>::kBlocks)) q4_tensor_k
       if (a.y_dtype == VSK_DTYPE_F32) put((float*)a.y, [](float v) { return v; });
       else if (a.y_dtype == VSK_DTYPE_F16) put((__half*)a.y, [](float v) { return __float2half_rn(v); });
       else put((__nv_bfloat16*)a.y, [](float v) { return __float2bfloat16_rn(v); });
+      if constexpr (MID) {   // (without middles both orders answer alike)
+        uint32_t wrong = 0;
+#pragma unroll
+        for (int q = 0; q < NV; ++q) wrong |= (q < nq && !isfinite(tot[q])) ? 1u << q : 0u;
+        for (; wrong; wrong &= wrong - 1) {
+          const int q = __ffs(wrong) - 1;
+          const float v = plain_product(a, a.vectors, row, q0 + q);
+          const int64_t at_y = (q0 + q) * a.y_stride + row;
+          if (a.y_dtype == VSK_DTYPE_F32) *VSK_CHK_W((float*)a.y + at_y) = v;
+          else if (a.y_dtype == VSK_DTYPE_F16) *VSK_CHK_W((__half*)a.y + at_y) = __float2half_rn(v);
+          else *VSK_CHK_W((__nv_bfloat16*)a.y + at_y) = __float2bfloat16_rn(v);
+        }
+      }
     }
 #pragma unroll
     for (int q = 0; q < NV; ++q) tot[q] = 0.f;
@@ -424,11 +439,14 @@ int32_t q4_product_tensor(Ctx* ctx, const vsk_q4_rows& rows, const void* x, int3
   a.scales = (const __half*)rows.scales;
   a.scale_stride = rows.scale_stride;
   a.n = rows.n;
+  a.dim = rows.dim;
+  a.group = rows.group;
   a.row_bytes = (rows.dim + 1) / 2;
   a.groups = (int)ceil_div(rows.dim, rows.group);
   a.steps = (int)ceil_div(rows.dim, 64);
   a.middles = (const __half*)rows.middles;
   a.quads = ((reinterpret_cast<uintptr_t>(rows.scales) | reinterpret_cast<uintptr_t>(rows.middles) | (uintptr_t)(2 * rows.scale_stride)) & 7) == 0;
+  a.vectors = Vectors{x, x_stride, x_dtype};
   a.nq = nq;
   a.y = y;
   a.y_stride = y_stride;
