@@ -11,6 +11,7 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -66,9 +67,49 @@ template <> __device__ __forceinline__ float lowest<float>() { return -CUDART_IN
 template <> __device__ __forceinline__ __half lowest<__half>() { return __ushort_as_half(0xfc00); }
 template <> __device__ __forceinline__ __nv_bfloat16 lowest<__nv_bfloat16>() { return __ushort_as_bfloat16(0xff80); }
 
-// A warp takes a.per_warp pieces of a row one after the other, the next one's loads under way.  32 x 8 x 131 072 bf16 logits (67 MB): 20 us,
-// 3.3 TB/s, issue slots 61 % busy: bound by the instructions of a logit (convert, maximum, convert, subtract, multiply, power, add).
+// Sixteen bytes of a row: elements at .. at + kVec - 1, -inf behind its end.  ALIGNED: the row begins at a 16-byte boundary.  Others are read as words
+// of four bytes; with 16-bit elements five of them, of which the first and the last count half where the row begins in the middle of a word.
+template <typename T, bool ALIGNED>
+struct RowVector {
+  static constexpr int kVec = 16 / (int)sizeof(T);
+  static constexpr bool kHalves = !ALIGNED && sizeof(T) == 2;
+  uint4 v;
+  uint32_t last;
+  // `shift`: bits of the row's first word that are not its own (shift_of)
+  __device__ __forceinline__ void load(const T* row, int64_t at, int64_t vocab, int shift) {
+    const int before = kHalves ? shift >> 4 : 0;
+    if (at >= before && at + kVec + (kHalves ? 2 : 0) <= vocab) {
+      if constexpr (ALIGNED) {
+        v = __ldg(reinterpret_cast<const uint4*>(row + at));
+      } else {
+        const uint32_t* const w = reinterpret_cast<const uint32_t*>(row + (at - before));
+        v = make_uint4(__ldg(w), __ldg(w + 1), __ldg(w + 2), __ldg(w + 3));
+        if constexpr (kHalves) last = __ldg(w + 4);
+      }
+    } else {
+      __align__(16) T h[kVec];
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) h[j] = at + j < vocab ? *VSK_CHK(row + at + j) : lowest<T>();
+      v = *reinterpret_cast<const uint4*>(h);
+      if constexpr (kHalves) {   // as if they had been read like that
+        last = __funnelshift_l(v.w, 0u, shift);
+        v = make_uint4(v.x << shift, __funnelshift_l(v.x, v.y, shift), __funnelshift_l(v.y, v.z, shift), __funnelshift_l(v.z, v.w, shift));
+      }
+    }
+  }
+  __device__ __forceinline__ uint4 whole(int shift) const {
+    if constexpr (!kHalves) return v;
+    else return make_uint4(__funnelshift_r(v.x, v.y, shift), __funnelshift_r(v.y, v.z, shift), __funnelshift_r(v.z, v.w, shift), __funnelshift_r(v.w, last, shift));
+  }
+};
 template <typename T>
+__device__ __forceinline__ int shift_of(const T* row) { return (int)(reinterpret_cast<uintptr_t>(row) & 2) * 8; }
+
+// A warp takes a.per_warp pieces of a row one after the other, the next one's loads under way.  Pieces are counted from the row's first logit, and
+// which of its logits a lane adds never changes: equal rows have equal sums, bit for bit, at whatever addresses they lie.
+// 32 x 8 x 131 072 bf16 logits (67 MB): 20 us, 3.3 TB/s, issue slots 61 % busy: bound by the instructions of a logit (convert, maximum,
+// convert, subtract, multiply, power, add).  ALIGNED: all rows begin at 16-byte boundaries.
+template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256) beam_pieces_kernel(const BeamArgs a) {
   constexpr int kVec = 16 / sizeof(T), kLoads = kPiece / (32 * kVec);
   let_the_next_launch_begin();
@@ -79,31 +120,19 @@ __global__ void __launch_bounds__(256) beam_pieces_kernel(const BeamArgs a) {
   const int64_t b = a.first_batch + blockIdx.z, row = b * a.beams + blockIdx.y;
   if (!isfinite(__ldg(a.scores + row)) || (a.finished && __ldg(a.finished + row))) return;   // not looked at again
   const T* base = reinterpret_cast<const T*>(a.logits) + b * a.batch_stride + blockIdx.y * a.beam_stride;
-  // pieces begin at 16-byte boundaries of the address, so the first one of a row may begin before it
-  const int before = (int)((reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T));
-  auto load = [&](int p, uint4 (&raw)[kLoads]) {
-    const int64_t first = (int64_t)p * kPiece - before + lane * kVec;
-    const T* src = base + first;
+  const int shift = shift_of(base);
+  RowVector<T, ALIGNED> next[kLoads];
+  auto load = [&](int p) {
+    const int64_t first = (int64_t)p * kPiece + lane * kVec;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int64_t at = first + i * 32 * kVec;
-      if (at >= 0 && at + kVec <= a.vocab) {
-        raw[i] = __ldg(reinterpret_cast<const uint4*>(src + i * 32 * kVec));
-      } else {
-        __align__(16) T h[kVec];
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) h[j] = at + j >= 0 && at + j < a.vocab ? *VSK_CHK(base + at + j) : lowest<T>();
-        raw[i] = *reinterpret_cast<const uint4*>(h);
-      }
-    }
+    for (int i = 0; i < kLoads; ++i) next[i].load(base, first + i * 32 * kVec, a.vocab, shift);
   };
-  uint4 next[kLoads];
-  load(piece, next);
+  load(piece);
   for (; piece < end; ++piece) {
     uint4 raw[kLoads];
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) raw[i] = next[i];
-    if (piece + 1 < end) load(piece + 1, next);
+    for (int i = 0; i < kLoads; ++i) raw[i] = next[i].whole(shift);
+    if (piece + 1 < end) load(piece + 1);
     float own[kLoads], top = -CUDART_INF_F;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
@@ -380,21 +409,25 @@ __global__ void __launch_bounds__(THREADS) beam_choose_kernel(const BeamArgs a) 
           continue;
         }
         const T* row = base + j * a.beam_stride;
-        const int64_t first = (int64_t)(at % pieces) * kPiece - (int64_t)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+        const int64_t first = (int64_t)(at % pieces) * kPiece;
         const int l0 = a.parts ? (int)(i % per_piece) : 0, l1 = a.parts ? l0 + 1 : kParts;
+        const bool aligned = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
+        const int shift = shift_of(row);
 #pragma unroll 4
         for (int l = l0; l < l1; ++l) {
           const int64_t v0 = first + (l * 32 + lane) * kVec;
-          float x[kVec];
-          if (v0 >= 0 && v0 + kVec <= a.vocab) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + v0));
-            const T* h = reinterpret_cast<const T*>(&u);
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) x[e] = as_float<T>(h[e]);
+          uint4 u;
+          if (aligned && v0 + kVec <= a.vocab) {
+            u = __ldg(reinterpret_cast<const uint4*>(row + v0));
           } else {
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) x[e] = v0 + e >= 0 && v0 + e < a.vocab ? as_float<T>(*VSK_CHK(row + v0 + e)) : -CUDART_INF_F;
+            RowVector<T, false> r;
+            r.load(row, v0, a.vocab, shift);
+            u = r.whole(shift);
           }
+          const T* h = reinterpret_cast<const T*>(&u);
+          float x[kVec];
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) x[e] = as_float<T>(h[e]);
           float top = x[0];
 #pragma unroll
           for (int e = 1; e < kVec; ++e) top = fmaxf(top, x[e]);
@@ -452,8 +485,8 @@ __global__ void __launch_bounds__(THREADS) beam_choose_kernel(const BeamArgs a) 
       const unsigned at = (unsigned)chosen[i / kPiece];
       const int j = (int)(at / pieces), p = (int)(at % pieces), e = (int)(i % kPiece);
       if (kind[j] == 2) return e == 0 ? Key{score[j], j * a.vocab + a.end_token} : no_key();
-      const int64_t v = (int64_t)p * kPiece + e - (int64_t)((reinterpret_cast<uintptr_t>(base + j * a.beam_stride) & 15) / sizeof(T));
-      return v >= 0 && v < a.vocab ? token_key(j, v, as_float<T>(*VSK_CHK(base + j * a.beam_stride + v))) : no_key();
+      const int64_t v = (int64_t)p * kPiece + e;
+      return v < a.vocab ? token_key(j, v, as_float<T>(*VSK_CHK(base + j * a.beam_stride + v))) : no_key();
     });
   }
   for (int r = threadIdx.x; r < a.k; r += THREADS) put(r, r < found ? list[r] : no_key());
@@ -470,7 +503,7 @@ int32_t select(Ctx* ctx, BeamArgs a) {
     return VSK_OK;
   }
   constexpr int kParts = kPiece * (int)sizeof(T) / 512;
-  a.pieces = (int)ceil_div(a.vocab + 16 / (int)sizeof(T) - 1, kPiece);
+  a.pieces = (int)ceil_div(a.vocab, kPiece);
   const int64_t items = a.batch * a.beams * a.pieces;
   // Parts of pieces where whole ones are few against k: the bound then leaves fewer candidates.  Four rows of 50 000, k = 64: 48 us with
   // parts, 180 without (more candidates than a list orders); 64 beams of 65 536, k = 128: 119 and 93.
@@ -481,10 +514,12 @@ int32_t select(Ctx* ctx, BeamArgs a) {
   a.parts = parts ? (float*)(a.stats + items) : nullptr;
   // as many pieces per warp as leave two rounds of warps (32 x 8 x 131 072 fp32: 84 us, one piece each: 87)
   a.per_warp = (int)std::max<int64_t>(1, std::min<int64_t>(8, items / ((int64_t)ctx->prop.multiProcessorCount * 64)));
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(a.logits) |
+                         (uintptr_t)((int64_t)sizeof(T) * ((a.batch > 1 ? a.batch_stride : 0) | (a.beams > 1 ? a.beam_stride : 0)));
+  auto* const pieces_kernel = (bits & 15) == 0 ? beam_pieces_kernel<T, true> : beam_pieces_kernel<T, false>;
   for (int64_t f = 0; f < a.batch; f += 65535) {
     a.first_batch = f;
-    beam_pieces_kernel<T><<<dim3((unsigned)ceil_div(a.pieces, 8 * a.per_warp), (unsigned)a.beams, (unsigned)std::min<int64_t>(65535, a.batch - f)), 256, 0,
-                           ctx->stream>>>(a);
+    pieces_kernel<<<dim3((unsigned)ceil_div(a.pieces, 8 * a.per_warp), (unsigned)a.beams, (unsigned)std::min<int64_t>(65535, a.batch - f)), 256, 0, ctx->stream>>>(a);
     ctx->stats.kernel_launches++;
     VSK_CUDA(ctx, cudaGetLastError());
   }
