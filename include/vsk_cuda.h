@@ -594,8 +594,9 @@ int32_t vsk_beam_select_dev(vsk_ctx* ctx, const void* logits, int32_t dtype, int
                             int64_t* out_tokens);
 /* The beams' states (key-value caches, token histories) moved after their parents, all states in one launch or a few:
  * row (b, i) of dst becomes row (b, parents[b][i]) of src; with parent -1 the row is left as it is.  dst = src (and the
- * same strides): in place, in any permutation.  Otherwise dst must not overlap any src, and no two states the same
- * memory.  A row is `outer` parts of steps * step_bytes contiguous bytes.  timed != 0: steps are time steps, and only the
+ * same strides): in place, in any permutation.  Otherwise dst must not overlap any src; no two dst overlap, and no two rows
+ * or parts of one.  Such states are refused; those that lie between one another are not.
+ * A row is `outer` parts of steps * step_bytes contiguous bytes.  timed != 0: steps are time steps, and only the
  * first lengths[b] of them move (lengths NULL: all); the bytes behind are left as they are.
  * A parent outside [-1, beams) leaves all states of its batch entry as they are and returns VSK_ERR_INVALID_INPUT.
  * parents and lengths are read throughout the call: memory between a dst's first and last byte is refused for them. */

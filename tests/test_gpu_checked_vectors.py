@@ -9,7 +9,8 @@ import pytest
 pytestmark = pytest.mark.gpu
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CHECKED = os.environ.get("VSK_CHECKED", "0") not in ("", "0")
-SUITES = ["tests/test_gpu_int4_vectors.py", "tests/test_gpu_beam_rows.py"]
+SUITES = ["tests/test_gpu_int4_vectors.py", "tests/test_gpu_beam_rows.py",
+          "tests/test_gpu_beam_states.py"]
 
 
 @pytest.mark.skipif(CHECKED, reason="this is the child process")

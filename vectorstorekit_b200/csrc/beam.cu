@@ -11,9 +11,11 @@
 #include <math_constants.h>
 
 #include <algorithm>
-#include <type_traits>
+#include <new>
+#include <vector>
 
 #include "common.cuh"
+#include "strided.cuh"
 
 namespace vsk {
 namespace {
@@ -651,6 +653,43 @@ int32_t reorder(Ctx* ctx, StateArgs& a, bool in_place, int64_t blocks) {
   return VSK_OK;
 }
 
+// No memory is written that another row, part or state is read from or written to: blocks move them in any order.
+int32_t check_apart(Ctx* ctx, const vsk_state* states, int32_t count, int64_t rows) {
+  struct Range {
+    Strided of;
+    int32_t state;
+    bool written;
+  };
+  std::vector<Range> ranges;
+  ranges.reserve(2 * (size_t)count);
+  for (int32_t i = 0; i < count; ++i) {
+    const vsk_state& s = states[i];
+    const int64_t inner = s.steps * s.step_bytes, src_part = s.outer > 1 ? s.src_outer_stride : 0, dst_part = s.outer > 1 ? s.dst_outer_stride : 0;
+    for (const auto& [row, part] : {std::pair{s.src_row_stride, src_part}, std::pair{s.dst_row_stride, dst_part}})
+      if ((double)rows * (double)row + (double)s.outer * (double)part > 0x1p60) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "state %d is too large", i);
+    ranges.push_back({{(int64_t)s.dst, rows, s.dst_row_stride, s.outer, dst_part, inner}, i, true});
+    if (meets_itself(ranges.back().of)) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "state %d: rows overlap", i);
+    if (s.src != s.dst) ranges.push_back({{(int64_t)s.src, rows, s.src_row_stride, s.outer, src_part, inner}, i, false});
+  }
+  std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.of.at < b.of.at; });
+  // Rows side by side in wider ones (a model's caches in one block) lie apart from one another as soon as each begins behind the one before it
+  // and the last ends before the first's next row: only what is behind such a run is looked at pair by pair.
+  for (size_t first = 0, behind; first < ranges.size(); first = behind) {
+    const int64_t row = ranges[first].of.row, next_row = ranges[first].of.at + row;
+    for (behind = first + 1; behind < ranges.size(); ++behind) {
+      const Strided &a = ranges[behind - 1].of, &b = ranges[behind].of;
+      if (b.row != row || b.at < a.at + a.in_row() || b.at + b.in_row() > next_row) break;
+    }
+    for (size_t i = first; i < behind; ++i) {
+      const int64_t end = ranges[i].of.last();
+      for (size_t j = behind; j < ranges.size() && ranges[j].of.at < end; ++j)
+        if ((ranges[i].written || ranges[j].written) && meet(ranges[i].of, ranges[j].of))
+          return fail(ctx, VSK_ERR_INVALID_INPUT, "memory of states %d and %d overlaps", ranges[i].state, ranges[j].state);
+    }
+  }
+  return VSK_OK;
+}
+
 int32_t check_ctx(vsk_ctx* c, Ctx** ctx) {
   *ctx = reinterpret_cast<Ctx*>(c);
   if (!*ctx) return VSK_ERR_INVALID_INPUT;
@@ -736,9 +775,11 @@ int32_t vsk_reorder_states_dev(vsk_ctx* c, const vsk_state* states, int32_t coun
     };
     if (inside(parents, batch * beams) || inside(lengths, batch))
       return fail(ctx, VSK_ERR_INVALID_INPUT, "parents or lengths lie in state %d, which moves", i);
-    for (int32_t j = 0; j < i; ++j)
-      if (states[j].dst == s.dst || states[j].src == s.dst || s.src == states[j].dst)
-        return fail(ctx, VSK_ERR_INVALID_INPUT, "states %d and %d are the same memory", j, i);
+  }
+  try {
+    VSK_TRY(check_apart(ctx, states, count, batch * beams));
+  } catch (const std::bad_alloc&) {
+    return fail(ctx, VSK_ERR_OUT_OF_MEMORY, "out of host memory");
   }
   drain_stale_error("vsk_reorder_states_dev");
   VSK_TRY(pinned_reserve(ctx, &ctx->host_flags[0], sizeof(int)));
