@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CHECKED = os.environ.get("VSK_CHECKED", "0") not in ("", "0")
 SUITES = ["tests/test_gpu_int4_vectors.py", "tests/test_gpu_beam_rows.py",
-          "tests/test_gpu_beam_states.py"]
+          "tests/test_gpu_beam_states.py", "tests/test_gpu_int4_sizes.py"]
 
 
 @pytest.mark.skipif(CHECKED, reason="this is the child process")

@@ -246,12 +246,16 @@ int32_t check_ctx(vsk_ctx* c, Ctx** ctx) {
   return VSK_OK;
 }
 
+// Elements of one array, and bytes that rows reach over: no size in bytes is computed past 64 bits.
+constexpr int64_t kMost = 1ll << 56;
+
 int32_t check_shape(Ctx* ctx, int64_t n, int32_t dim, int32_t group) {
   if (n <= 0) return fail(ctx, VSK_ERR_EMPTY_INPUT, "no rows");
   if (n > (1ll << 40)) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "too many rows");
   if (dim <= 0 || dim > (1 << 24)) return fail(ctx, VSK_ERR_DIMENSION_MISMATCH, "dimension must be in [1, 2^24]");
   if (group != 32 && group != 64 && group != 128)
     return fail(ctx, VSK_ERR_UNSUPPORTED_OPERATION, "groups of %d columns are not supported (32, 64 or 128)", group);
+  if (n > kMost / dim) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "too many rows of %d columns", dim);
   return VSK_OK;
 }
 
@@ -261,6 +265,8 @@ int32_t check_rows(Ctx* ctx, const vsk_q4_rows* r) {
   if (!r->codes || !r->scales) return fail(ctx, VSK_ERR_INVALID_INPUT, "null codes or scales");
   if (r->code_stride < ((int64_t)r->dim + 1) / 2) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "code rows are shorter than %d columns", r->dim);
   if (r->scale_stride < ceil_div(r->dim, r->group)) return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "scale rows are shorter than the groups of %d columns", r->dim);
+  if (r->n > 1 && std::max(r->code_stride, r->scale_stride) > kMost / r->n)
+    return fail(ctx, VSK_ERR_INVALID_BUFFER_SIZE, "the distance of code or scale rows is too large");
   if ((reinterpret_cast<uintptr_t>(r->scales) & 1) || (reinterpret_cast<uintptr_t>(r->middles) & 1))
     return fail(ctx, VSK_ERR_INVALID_INPUT, "scales and middles must be aligned to two bytes");
   return VSK_OK;
