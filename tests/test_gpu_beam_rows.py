@@ -55,3 +55,14 @@ def test_totals_do_not_depend_on_the_address(engine, dtype, normalize):
                 wide[:, :, at:at + vocab] = x
                 got = engine.selectBeams(wide[:, :, at:at + vocab], scores, k, normalize=normalize)
                 assert all(torch.equal(a, b) for a, b in zip(first, got)), (vocab, pad, at)
+
+
+def test_an_end_token_outside_the_vocabulary_is_refused_however_large(engine):
+    import torch
+    import vectorstorekit_b200 as vsk
+    x, scores, finished = torch.zeros((1, 2, 100), device="cuda"), torch.zeros((1, 2), device="cuda"), torch.ones((1, 2), dtype=torch.bool, device="cuda")
+    for end in (100, -1, 2 ** 64 + 3, -2 ** 64 + 3, 2 ** 200):
+        with pytest.raises(vsk.InvalidInput):
+            engine.selectBeams(x, scores, 2, finished=finished, end_token=end)
+        assert engine.selectBeams(x, scores, 2, end_token=end)[2].tolist() == [[0, 1]]      # nobody has finished
+    assert engine.selectBeams(x, scores, 2, finished=finished, end_token=99)[2].tolist() == [[99, 99]]

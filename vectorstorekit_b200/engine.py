@@ -542,9 +542,11 @@ class CUDAAccelerationEngine:
             raise InvalidInput("scores must be a CUDA tensor of float32")
         if finished is not None and (not _is_dev(finished) or finished.dtype not in (torch.bool, torch.uint8)):
             raise InvalidInput("finished must be a CUDA tensor of bool")
-        k = int(k)
+        k, end_token = int(k), int(end_token)
         if not 1 <= k <= 128:
             raise InvalidInput("k must be in [1, 128]")
+        if finished is not None and not 0 <= end_token < v:   # (here: the library's argument has 64 bits)
+            raise InvalidInput(f"the end token must be in [0, {v})")
         per_batch, per_beam, step = logits.stride()
         if v > 1 and step != 1:
             logits = logits.contiguous()
@@ -555,7 +557,7 @@ class CUDAAccelerationEngine:
         places = torch.empty((2, b, k), dtype=torch.int64, device=logits.device)
         beams, tokens = places.unbind(0)
         pl, ps, pf, po, pp = _device_pointers(self.dev, logits, scores, finished, out, places)
-        self.dev.check(self._lib.vsk_beam_select_dev(self.dev._h, pl, kind, b, w, v, per_batch, per_beam, ps, pf, int(end_token),
+        self.dev.check(self._lib.vsk_beam_select_dev(self.dev._h, pl, kind, b, w, v, per_batch, per_beam, ps, pf, end_token if finished is not None else 0,
                                                      1 if normalize else 0, k, po, pp, pp + 8 * b * k))
         return out, beams, tokens
 
