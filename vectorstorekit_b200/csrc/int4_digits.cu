@@ -4,7 +4,7 @@
 // clock.  A code in the high half of a byte, its top bit turned, IS the signed byte 16 (code - 8): eight codes take three
 // instructions, a third of what any 16-bit form takes.  So x comes in whole numbers too.  Each vector is scaled by a power of two until
 // its largest element fills four signed bytes and rounded there, by at most 2^-31 of that element: an fp32 sum that contains it rounds by
-// a hundred times as much.  The bytes are columns of their own in m16n8k32 products, a tile of eight holds two vectors; group sums are exact
+// a hundred times as much.  (A row with no weight there sees that rounding alone: elements below it are lost to such a row.)  The bytes are columns of their own in m16n8k32 products, a tile of eight holds two vectors; group sums are exact
 // whole numbers, become fp32 (a magic constant is the products' starting value: its difference is the number) and meet the scale there.
 // A vector with an infinity or a NaN has no such form: its products are taken one by one in fp32.
 //
@@ -265,11 +265,10 @@ __global__ void __launch_bounds__(32 * kWarps, DT == 4 ? 1 : 2) q4_digits_kernel
   const int magic[4] = {kMagic, kMagic, kMagic, kMagic};
   const f32x2 less = pair_of(-12582912.f, -12582912.f);
   int slot = 0;
-  constexpr bool kAhead = true;
-  uint4 x[DT][2], x_next[kAhead ? DT : 1][2];
+  uint4 x[DT][2], x_next[DT][2];
   const uint4* step = frags;
   int x_k = k0;
-  auto read_digits = [&](auto& to) {
+  auto read_digits = [&](uint4 (&to)[DT][2]) {
 #pragma unroll
     for (int j = 0; j < DT; ++j)
 #pragma unroll
@@ -280,7 +279,7 @@ __global__ void __launch_bounds__(32 * kWarps, DT == 4 ? 1 : 2) q4_digits_kernel
       step = frags;
     }
   };
-  if constexpr (kAhead) read_digits(x_next);
+  read_digits(x_next);
   for (int tile = tile0; tile < tiles; tile += stride) {
     f32x2 tot[2][DT][2];   // digits 8 j + 2 t and the next of rows 16 i + g and 8 more
     float mid[S::kVectors];
@@ -295,15 +294,11 @@ __global__ void __launch_bounds__(32 * kWarps, DT == 4 ? 1 : 2) q4_digits_kernel
     const float* sums = MID ? a.sums + q0 * a.sum_stride + k0 * GW : nullptr;
 #pragma unroll 1
     for (int k = k0; k < k1; ++k) {
-      if constexpr (kAhead) {
 #pragma unroll
-        for (int j = 0; j < DT; ++j)
+      for (int j = 0; j < DT; ++j)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) x[j][h] = x_next[j][h];
-        read_digits(x_next);
-      } else {
-        read_digits(x);
-      }
+        for (int h = 0; h < 2; ++h) x[j][h] = x_next[j][h];
+      read_digits(x_next);
       read_scales(after);
 
       copy_wait<S::kStages - 2>();

@@ -104,8 +104,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 4 ? 1 : 2) q4_product_kerne
   const int k0 = a.ksteps * wk / team, k1 = a.ksteps * (wk + 1) / team;
   const int row_bytes = (a.dim + 1) / 2;
 
-  // the codes of one step after the other: this lane's rows (eight apart) and its place in them.  Rows behind the last one repeat it, bytes
-  // behind a row's end are zeros: their digits are.
+  // the codes of one step after the other: this lane's rows (eight apart) and its place in them.  Rows behind the last one repeat it; bytes
+  // behind a row's end are zeros, and so are the vectors' columns there.
   const int f_piece = lane & 3;
   const uint8_t* f_src[WIDE ? 4 : 1];
   int f_tile = tile0, f_k = k0, f_slot = 0;
