@@ -551,8 +551,10 @@ int32_t vsk_pq_index_add_dev(vsk_index* index, const uint8_t* codes, int64_t n);
  *   product     y[q * y_stride + r] = sum over the columns of value(r, i) x[q * x_stride + i]: the scores of nq vectors
  *               against all rows, as a decoding step takes them from a projection or an output head, or a query from a store
  *               (dotProduct negates them).  Sums in fp32, rounded once to y's type.  fp32 vectors, and up to four 16-bit ones,
- *               are taken to 2^-31 of their largest element, others exactly.  Elements below 2^120; an infinity or a NaN stays in
- *               its vector's products.  x and y must not overlap. */
+ *               are taken to 2^-31 of their largest element (a row without weight there loses what lies below that), others exactly.
+ *               The same call gives the same bits; the order of the sums, and with it their last bits, depends on the numbers of
+ *               rows and vectors.  Elements below 2^120; an infinity or a NaN stays in its vector's products, which are what the
+ *               formula gives.  At most 524 280 fp32 vectors, 2 097 120 16-bit ones.  x and y must not overlap. */
 typedef enum vsk_dtype { VSK_DTYPE_F32 = 0, VSK_DTYPE_F16 = 1, VSK_DTYPE_BF16 = 2 } vsk_dtype;
 typedef struct vsk_q4_rows {
   const uint8_t* codes;
@@ -582,7 +584,9 @@ int32_t vsk_q4_product_dev(vsk_ctx* ctx, const vsk_q4_rows* rows, const void* x,
  *   total       scores[b][j] + logit - log(sum of exp of the row)   normalize != 0; a row of which that sum is zero or
  *                                                                   not a number (a NaN or +inf in it) offers nothing
  *               scores[b][j] + logit                                otherwise
- *               in 64 bits; equal totals are ordered by (beam, token)
+ *               added and compared in 64 bits; equal totals are ordered by (beam, token).  The log of a row's sum comes from
+ *               exponentials and partial sums in fp32, within 1e-5 of it: totals of DIFFERENT beams that lie nearer than
+ *               twice that may change places.  Equal rows have equal logs, at whatever addresses they lie
  *   finished    [batch][beams] bytes or NULL: such a beam offers (end_token, at its own score) and nothing else; its
  *               logits are not read
  *   out         [batch][k] totals rounded to fp32, descending, with their beams and tokens; places without a candidate have

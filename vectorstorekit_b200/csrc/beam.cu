@@ -463,7 +463,8 @@ __global__ void __launch_bounds__(THREADS) beam_choose_kernel(const BeamArgs a) 
     return;
   }
 
-  // Many equal totals, or many candidates in few places: exact keys throughout.
+  // Many equal totals, many candidates in few places, or hardly more parts than k (every candidate reaches the bound then: one row of 8 000 with
+  // k = 64 takes 90 us with cold caches, four of 32 768 with k = 8 take 46): exact keys throughout.
   int found;
   __syncthreads();
   if constexpr (SMALL) {

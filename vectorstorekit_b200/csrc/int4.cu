@@ -26,8 +26,8 @@ template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat
 // ---- encoding -----------------------------------------------------------------------------------------------------------
 // Eight columns per lane: a group of G columns is G / 8 lanes, its extremes a few shuffles.  `lanes` neighbouring lanes share a row (short
 // rows leave several to a warp) and walk along it, the next columns' load under way.  100 000 x 768 fp32, groups of 32, min / max
-// (307 MB in): 93 us, issue slots 84 % busy: bound by the instructions of a value, of which the 64-bit ones are kept to what the
-// definition needs.
+// (307 MB in): 93 us, issue slots 84 % busy: bound by the instructions of a value and of its group's scale, which every lane of the group makes (a few
+// of them in 64 bits; quotients in 64 bits are taken only next to a border).
 
 // (float)(d / 15) with the quotient in 64 bits.  The product with the rounded reciprocal is off by less than 2 of its last bits: it
 // rounds to the same fp32 number unless it lies that near to the middle between two.
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(256) q4_encode_kernel(const T* __restrict__ ro
   }
 }
 
-// ---- decoding: eight columns per thread, `lanes` threads along a row (100 000 x 768 to fp32, 307 MB out: 76 us, 4.8 TB/s) -------------------------------------------------------------
+// ---- decoding: eight columns per thread, `lanes` threads along a row (100 000 x 768 to fp32, 48 MB in and 307 MB out: 76 us, 4.7 TB/s asked for) -------
 constexpr int kDecodeSteps = 4;
 __global__ void __launch_bounds__(256) q4_decode_kernel(const uint8_t* __restrict__ codes, int64_t code_stride,
                                                         const __half* __restrict__ scales, const __half* __restrict__ middles,

@@ -15,7 +15,8 @@
 // Codes are never multiplied by a rounded weight: every product is exact, sums are fp32.
 //
 // 131 072 x 2 048, groups of 128, 32 bf16 vectors: the call takes 84 us, 127 with the warp form.  Bound by a step's chain (copies - numbers - tensor
-// memory - products - sums, about 0.6 us for a block alone, four blocks to an SM) and by 1 024 tiles on 592 blocks.  Codes to shared memory
+// memory - products - sums: 0.57 us for a block alone, 18 944 x 8 192 in 72.5 us; four blocks to an SM) and by 1 024 tiles on 592 blocks: kernel 61 us, issue
+// slots 59 %, tensor pipe 15 %.  Codes to shared memory
 // instead of tensor memory: 97 against 93 us, then codes and vectors asked for through registers two and one steps ahead instead of copies: 93 against 84.
 #include "int4.cuh"
 #include "tc_ptx.cuh"

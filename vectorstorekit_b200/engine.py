@@ -522,8 +522,8 @@ class CUDAAccelerationEngine:
 
         ``logits [batch][beams][vocab]`` (float32, float16, bfloat16; any strides before a contiguous last axis) are an output head's,
         or the scores of the rows that a search found for each chain.  ``scores [batch][beams]`` (float32) are the beams' own.  With
-        ``normalize`` a continuation's total is score + logit - log(sum of exp of its row), without score + logit, in 64 bits.  -inf
-        and NaN are never chosen; a beam whose score is not finite offers nothing.  ``finished [batch][beams]`` (bool): such a
+        ``normalize`` a continuation's total is score + logit - log(sum of exp of its row), without score + logit, added and compared in
+        64 bits (the log to 1e-5: totals of different beams that lie nearer than twice that may change places).  -inf and NaN are never chosen; a beam whose score is not finite offers nothing.  ``finished [batch][beams]`` (bool): such a
         beam offers ``end_token`` at its own score and nothing else.  Places without a candidate: -inf, -1, -1.  At most 64 beams, ``k``
         at most 128.  CUDA tensors; no gradient flows."""
         if not _is_dev(logits):
@@ -565,7 +565,8 @@ class CUDAAccelerationEngine:
         """The beams' states moved after their parents: row ``b * beams + i`` of each result is row ``b * beams + parents[b][i]``.
 
         ``states``: CUDA tensors ``[batch * beams, ...]`` of any element type (key-value caches, token histories).  ``out=None`` moves
-        them in place, in any permutation; otherwise into the tensors of ``out`` (same shapes and types, other memory).  ``parents
+        them in place, in any permutation; otherwise into the tensors of ``out`` (same shapes and types, other memory: overlap is
+        refused, also between states that are written; they may lie between one another).  ``parents
         [batch][beams]`` int64, not in a moved state's memory; a parent of -1 leaves its row as it is.  ``lengths [batch]`` int64 with
         ``time_axis`` (one number, or one per state; None for a state without time): only the first ``lengths[b]`` places of that axis
         move, what lies behind stays.

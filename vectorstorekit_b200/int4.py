@@ -118,7 +118,8 @@ class Int4Quantizer:
         """``[queries][n]`` products of vectors ``x [queries][dim]`` with all rows: the logits of an output head, a projection of
         tokens, or the scores of queries against a store (``DistanceMetric.dotProduct`` is their negative).  Sums in fp32, rounded
         once to ``out_dtype`` (float32, float16 or bfloat16; default: x's type).  fp32 vectors, and up to four 16-bit ones, are taken to
-        2^-31 of their largest element, others exactly.  CUDA tensors; no gradient flows."""
+        2^-31 of their largest element, others exactly; the order of the sums depends on the numbers of rows and vectors.  CUDA tensors;
+        no gradient flows."""
         if not _is_dev(x):
             raise InvalidInput("product takes CUDA tensors")
         if x.dim() != 2:
